@@ -394,6 +394,76 @@ int pfa_ct_lincomb(const pfa_context *ctx, size_t L, size_t size, size_t ct_size
                    const size_t *in_limbs, const int64_t *consts, size_t n, const uint64_t *bias, uint64_t *out,
                    void *stream);
 
+/* ------------------------------------------------- the clear end of a step
+ *
+ * No reference counterpart as kernels (its client runs these on the CPU).  What
+ * the holder of the key computes from decrypted hidden states: norm, products
+ * with clear weights, probabilities and the choice of tokens.  None takes a
+ * context; they run on the current device, on `stream`, and allocate nothing.
+ * Rows are contiguous, `*_stride` elements apart. */
+
+/* element types of floating tensors */
+#define PFA_F32 0
+#define PFA_BF16 1
+#define PFA_F16 2
+
+/* Rows of x [rows][width] as codes of 8 bits: scale = max|x| / 127, code =
+ * x / scale rounded to the nearest integer, ties to even.  A row of zeros has
+ * scale 0 and codes 0; a row with a NaN or an infinity has scale NaN and codes 0. */
+int pfa_quantize_int8(const void *x, size_t x_stride, int type, size_t rows, size_t width, int8_t *codes,
+                      size_t codes_stride, float *scales, void *stream);
+
+/* y = x + residual (residual NULL: y = x), total = y rounded to `type` (written
+ * only with a residual), then the codes and scales (as pfa_quantize_int8) of
+ * y / sqrt(mean(y^2) + eps) * weight, from the unrounded y.  weight [width].  A
+ * row whose sum of squares is not finite has scale NaN and codes 0.  total may be
+ * x or residual. */
+int pfa_rms_norm_int8(const void *x, size_t x_stride, const void *residual, size_t residual_stride,
+                      const void *weight, int type, size_t rows, size_t width, double eps, void *total,
+                      size_t total_stride, int8_t *codes, size_t codes_stride, float *scales, void *stream);
+
+/* out[m][n] = (sum_k a[m][k] b[n][k]) a_scales[m] b_scales[n] + bias[n] (bias NULL:
+ * none), out of `type`.  a [M][K], b [N][K].  The sums are exact: K <= 131071.
+ * Rows of a and b that start at multiples of 16 bytes are read fastest.
+ * workspace: `workspace_bytes` of device memory, 16-byte aligned, that no other
+ * call in flight uses, or NULL and 0. */
+int pfa_int8_matmul(const int8_t *a, size_t a_stride, const float *a_scales, const int8_t *b, size_t b_stride,
+                    const float *b_scales, const float *bias, size_t M, size_t N, size_t K, void *out, int type,
+                    size_t out_stride, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Probabilities out [rows][vocab] of logits [rows][vocab]: softmax(logits /
+ * temperature) over the places where mask [rows][vocab] (bytes; mask_stride 0:
+ * one row for all; NULL: everywhere) is not 0; 0 elsewhere, whatever stands
+ * there.  A row's temperature is temperatures[row], or `temperature` where
+ * temperatures is NULL; at 0 the lowest place of the largest logit gets 1.  A row
+ * that allows nothing, or -infinity alone, is all 0.  A NaN or (above temperature
+ * 0) +infinity in an allowed place, or a negative or NaN temperature, makes the
+ * row's allowed places NaN.  workspace as in pfa_int8_matmul. */
+int pfa_token_probabilities(const void *logits, size_t stride, int type, size_t rows, size_t vocab,
+                            const float *temperatures, double temperature, const uint8_t *mask, size_t mask_stride,
+                            float *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Drafted tokens against the target's probabilities.  Of sequence b's
+ * lengths[b] drafts (NULL: K; clamped to 0..K) draft i is kept while
+ *   uniforms[b][i] draft[b][i][x_i] < target[b][i][x_i]
+ * (draft NULL: the drafts were certain, 1 in place of draft's value; a token
+ * outside the vocabulary is not kept).  At place n, the first not kept or the
+ * end, a token is drawn by noise [b][vocab], exponentially distributed: the
+ * lowest v with the largest w(v) / noise[b][v] among the positive w(v), with
+ *   w = max(target - draft, 0) at n after a refusal (draft NULL: target without x_n),
+ *   w = target at n at the end, or where the former leaves nothing;
+ * -1 if no weight is positive.  tokens [batch][K + 1]: the n kept drafts, the
+ * token drawn, then -1; accepted [batch]: n.  Tokens have token_bytes (4 or 8),
+ * lengths length_bytes.  uniforms [batch][K]; the strides are of target and draft
+ * (from sequence to sequence, from place to place) and of noise.  All arithmetic
+ * is in 32-bit floats, each operation rounded once.  workspace as in
+ * pfa_int8_matmul. */
+int pfa_verify_drafts(const void *drafts, int token_bytes, const void *lengths, int length_bytes, size_t batch,
+                      size_t K, size_t vocab, const void *target, size_t target_batch, size_t target_place,
+                      const void *draft, size_t draft_batch, size_t draft_place, int type, const float *uniforms,
+                      const float *noise, size_t noise_batch, void *tokens, int32_t *accepted, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

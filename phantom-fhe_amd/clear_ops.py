@@ -1,0 +1,276 @@
+"""The clear end of an encrypted generation step, on the GPU.
+
+A server that evaluates a model under encryption hands back the ciphertext of a
+hidden state; only the holder of the key can turn it into an answer.  These are
+the operators the holder runs on decrypted states: the norm, products with clear
+weights in 8 bits, probabilities, and the check of drafted tokens (an encrypted
+pass takes so long that several drafted tokens are checked per pass).  Callers use
+them through pyPhantom, which re-exports them.
+
+They take torch tensors on a GPU, launch on torch's current stream of the tensors'
+device, return new tensors and never wait for the GPU.  Rows may be strided, the
+elements of a row are adjacent.  Wrong arguments raise ValueError, as everywhere in
+pyPhantom.  There is no CPU fallback.
+"""
+from __future__ import annotations
+
+import torch
+
+import pfa_native as _N
+
+__all__ = ["quantize_int8", "rms_norm_int8", "int8_matmul", "token_probabilities", "verify_drafts"]
+
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PFA_F32, PFA_BF16, PFA_F16
+_WHOLE = {torch.int32: 4, torch.int64: 8}
+
+
+def _fail(what):
+    raise ValueError(what)
+
+
+def _type_of(t, name):
+    code = _TYPE.get(t.dtype)
+    if code is None:
+        _fail(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _same_device(first, **others):
+    if not first.is_cuda:
+        _fail("expected tensors on a GPU")
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            _fail(f"{name} is on {t.device}, not on {first.device}")
+
+
+def _call(name, t, *args):
+    """The entry point on t's device and its current stream."""
+    device = t.device.index
+    if device == torch.cuda.current_device():
+        _N.call(name, *args, _N.stream_of(t))
+    else:
+        with torch.cuda.device(device):
+            _N.call(name, *args, _N.stream_of(t))
+
+
+def _matrix(t, name):
+    """t as (two-dimensional view of its rows, distance between them)."""
+    if t.dim() < 1:
+        _fail(f"{name} needs at least one dimension")
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1]) if t.numel() else t.new_empty((t.shape[:-1].numel(), t.shape[-1]))
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        _fail(f"{name}: the elements of a row must be adjacent")
+    if t.shape[0] > 1 and 0 < t.stride(0) < t.shape[1]:
+        _fail(f"{name}: rows overlap")
+    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(t, n, dtype, name):
+    if t.dtype != dtype or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        _fail(f"{name}: expected {n} adjacent values of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    return t
+
+
+def _new_codes(shape, device):
+    """Codes whose rows start at multiples of 16 bytes, which int8_matmul reads fastest."""
+    width = shape[-1]
+    if width % 16 == 0:
+        return torch.empty(shape, dtype=torch.int8, device=device)
+    return torch.empty((*shape[:-1], -(-width // 16) * 16), dtype=torch.int8, device=device)[..., :width]
+
+
+def quantize_int8(x):
+    """Codes of 8 bits of x [..., width], with one scale for each row: (codes int8
+    [..., width], scales float32 [...]), x ~ codes * scales.
+
+    scale = max|x| / 127, code = x / scale to the nearest, ties to even.  Rows of
+    zeros have scale 0; rows with a NaN or an infinity have scale NaN and codes 0.
+    For weights a row is an output channel, for activations a token.  Rows of the
+    codes start at multiples of 16 bytes (codes.stride() says where).
+    """
+    kind = _type_of(x, "x")
+    _same_device(x)
+    rows, stride = _matrix(x, "x")
+    codes = _new_codes(x.shape, x.device)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if scales.numel():
+        _call("pfa_quantize_int8", x, rows.data_ptr(), stride, kind, rows.shape[0], rows.shape[1], codes.data_ptr(),
+              _matrix(codes, "codes")[1], scales.data_ptr())
+    return codes, scales
+
+
+def rms_norm_int8(x, weight, eps=1e-6, residual=None):
+    """Root-mean-square norm of x + residual as codes of 8 bits: (codes int8 [..., width],
+    scales float32 [...], total).
+
+    With y = x + residual: total = y in x's type (x itself without a residual), and
+    codes, scales are quantize_int8's of y / sqrt(mean(y^2) + eps) * weight, formed from
+    the unrounded y.  x [..., width]; residual like x; weight [width]; all of one type.
+    """
+    kind = _type_of(x, "x")
+    _same_device(x, weight=weight, residual=residual)
+    if not eps >= 0:
+        _fail("eps must be 0 or more")
+    rows, stride = _matrix(x, "x")
+    n, width = rows.shape
+    if width == 0:
+        _fail("x: the mean of an empty row")
+    _vector(weight, width, x.dtype, "weight")
+    total, more, more_stride, total_stride = x, None, 0, 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            _fail(f"residual: expected {tuple(x.shape)} of {x.dtype}, got {tuple(residual.shape)} of {residual.dtype}")
+        more, more_stride = _matrix(residual, "residual")
+        total, total_stride = torch.empty(x.shape, dtype=x.dtype, device=x.device), width
+    codes = _new_codes(x.shape, x.device)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if n:
+        _call("pfa_rms_norm_int8", x, rows.data_ptr(), stride, more.data_ptr() if more is not None else None,
+              more_stride, weight.data_ptr(), kind, n, width, float(eps), total.data_ptr() if total_stride else None,
+              total_stride, codes.data_ptr(), _matrix(codes, "codes")[1], scales.data_ptr())
+    return codes, scales, total
+
+
+def int8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
+    """out[..., n] = (sum_k a[..., k] b[n, k]) a_scales[...] b_scales[n] + bias[n].
+
+    a int8 [..., K] with a_scales float32 [...] (one for each token), b int8 [N, K] with
+    b_scales float32 [N] (one for each output channel), as quantize_int8 gives them;
+    bias float32 [N]; out of out_dtype (float32, bfloat16 or float16).  The sums are
+    exact, so K is at most 131071; scales and bias are applied in 32 bits.  Rows of a
+    and b that start at multiples of 16 bytes are read fastest.
+    """
+    kind = _TYPE.get(out_dtype)
+    if kind is None:
+        _fail(f"out_dtype: expected float32, bfloat16 or float16, got {out_dtype}")
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        _fail(f"expected int8 codes, got {a.dtype} and {b.dtype}")
+    _same_device(a, a_scales=a_scales, b=b, b_scales=b_scales, bias=bias)
+    if b.dim() != 2 or a.dim() < 1 or a.shape[-1] != b.shape[1]:
+        _fail(f"shapes {tuple(a.shape)} and {tuple(b.shape)} do not multiply")
+    if a_scales.dtype != torch.float32 or a_scales.shape != a.shape[:-1] or not a_scales.is_contiguous():
+        _fail(f"a_scales: expected contiguous float32 {tuple(a.shape[:-1])}, got {tuple(a_scales.shape)} of "
+              f"{a_scales.dtype}")
+    rows, a_stride = _matrix(a, "a")
+    cols, b_stride = _matrix(b, "b")
+    m, k = rows.shape
+    n = cols.shape[0]
+    _vector(b_scales, n, torch.float32, "b_scales")
+    if bias is not None:
+        _vector(bias, n, torch.float32, "bias")
+    out = torch.empty((*a.shape[:-1], n), dtype=out_dtype, device=a.device)
+    if m and n:
+        _call("pfa_int8_matmul", a, rows.data_ptr(), a_stride, a_scales.data_ptr(), cols.data_ptr(), b_stride,
+              b_scales.data_ptr(), bias.data_ptr() if bias is not None else None, m, n, k, out.data_ptr(), kind, n,
+              None, 0)
+    return out
+
+
+def token_probabilities(logits, temperature=1.0, mask=None):
+    """softmax(logits / temperature) over the allowed places: float32 [..., vocab].
+
+    temperature: a number, or float32 [...] with one for each row; at 0 the lowest place
+    of the largest allowed logit gets 1.  mask: bool [vocab] or like logits, True where
+    a token is allowed; other places get 0 whatever their logits are.  A row that allows
+    nothing (or -infinity alone) is all 0.  A NaN, or above temperature 0 a +infinity, in
+    an allowed place and a negative or NaN temperature make a row's allowed places NaN.
+    """
+    kind = _type_of(logits, "logits")
+    rows, stride = _matrix(logits, "logits")
+    n, vocab = rows.shape
+    temperatures, one = None, 0.0
+    if isinstance(temperature, torch.Tensor):
+        if temperature.dtype != torch.float32 or temperature.shape != logits.shape[:-1] or \
+                not temperature.is_contiguous():
+            _fail(f"temperature: expected a number or contiguous float32 {tuple(logits.shape[:-1])}")
+        temperatures = temperature
+    else:
+        one = float(temperature)
+        if not 0 <= one < float("inf"):
+            _fail("the temperature must be 0 or more")
+    allowed, mask_stride = None, 0
+    if mask is not None:
+        if mask.dtype != torch.bool or (mask.shape != logits.shape and mask.shape != (vocab,)):
+            _fail(f"mask: expected bool of {tuple(logits.shape)} or ({vocab},), got {tuple(mask.shape)} of "
+                  f"{mask.dtype}")
+        if mask.dim() == 1 and vocab > 1 and mask.stride(0) != 1:
+            _fail("mask: the places of a row must be adjacent")
+        if mask.shape == logits.shape and logits.dim() > 1:
+            allowed, mask_stride = _matrix(mask, "mask")
+        else:
+            allowed = mask
+    _same_device(logits, temperature=temperatures, mask=mask)
+    out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+    if out.numel():
+        _call("pfa_token_probabilities", logits, rows.data_ptr(), stride, kind, n, vocab,
+              temperatures.data_ptr() if temperatures is not None else None, one,
+              allowed.data_ptr() if allowed is not None else None, mask_stride, out.data_ptr(), None, 0)
+    return out
+
+
+def verify_drafts(draft_tokens, target_probs, uniforms, noise, draft_probs=None, lengths=None):
+    """Drafted tokens against the target's probabilities, by given random numbers:
+    (tokens [batch, drafts + 1], accepted int32 [batch]).
+
+    draft_tokens int32 or int64 [batch, drafts]; target_probs [batch, drafts + 1, vocab];
+    draft_probs [batch, drafts, vocab] of the same type, or None where the drafts were
+    certain (chosen without chance); uniforms float32 [batch, drafts] in [0, 1); noise
+    float32 [batch, vocab], exponentially distributed; lengths int32 or int64 [batch]: how
+    many drafts a sequence has, where not all.
+
+    A draft x is kept while uniform * draft_probs[x] < target_probs[x]; a token outside the
+    vocabulary is not.  At the first refusal a token is drawn from max(target - draft, 0),
+    at the end of the drafts from target: the one with the largest weight / noise (the
+    lowest among equals), whose distribution is the weights'.  So the tokens are distributed
+    as if the target had drawn them one by one.  `tokens` are the kept drafts, that
+    token, then -1; `accepted` counts the kept drafts.  Where the difference leaves
+    nothing, target is taken; where no weight is positive, the token is -1.  With 0 drafts
+    this draws one token for each sequence.
+    """
+    kind = _type_of(target_probs, "target_probs")
+    size = _WHOLE.get(draft_tokens.dtype)
+    if size is None:
+        _fail(f"draft_tokens: expected int32 or int64, got {draft_tokens.dtype}")
+    _same_device(target_probs, draft_tokens=draft_tokens, uniforms=uniforms, noise=noise, draft_probs=draft_probs,
+                 lengths=lengths)
+    if target_probs.dim() != 3 or target_probs.shape[1] < 1:
+        _fail(f"target_probs: expected [batch, drafts + 1, vocab], got {tuple(target_probs.shape)}")
+    batch, places, vocab = target_probs.shape
+    drafts = places - 1
+
+    def place(t, name):
+        if vocab > 1 and t.stride(2) != 1:
+            _fail(f"{name}: the probabilities of a place must be adjacent")
+        return t.stride(0), t.stride(1)
+
+    if draft_tokens.shape != (batch, drafts) or not draft_tokens.is_contiguous():
+        _fail(f"draft_tokens: expected contiguous {(batch, drafts)}, got {tuple(draft_tokens.shape)}")
+    if uniforms.dtype != torch.float32 or uniforms.shape != (batch, drafts) or not uniforms.is_contiguous():
+        _fail(f"uniforms: expected contiguous float32 {(batch, drafts)}, got {tuple(uniforms.shape)} of "
+              f"{uniforms.dtype}")
+    if noise.dtype != torch.float32 or noise.shape != (batch, vocab) or (vocab > 1 and noise.stride(1) != 1):
+        _fail(f"noise: expected float32 {(batch, vocab)} with adjacent elements, got {tuple(noise.shape)} of "
+              f"{noise.dtype}")
+    target_batch, target_place = place(target_probs, "target_probs")
+    draft_batch = draft_place = 0
+    if draft_probs is not None:
+        if draft_probs.shape != (batch, drafts, vocab) or draft_probs.dtype != target_probs.dtype:
+            _fail(f"draft_probs: expected {(batch, drafts, vocab)} of {target_probs.dtype}, got "
+                  f"{tuple(draft_probs.shape)} of {draft_probs.dtype}")
+        draft_batch, draft_place = place(draft_probs, "draft_probs")
+    length_size = 4
+    if lengths is not None:
+        length_size = _WHOLE.get(lengths.dtype)
+        if length_size is None or lengths.shape != (batch,) or not lengths.is_contiguous():
+            _fail(f"lengths: expected {batch} adjacent values of int32 or int64, got {tuple(lengths.shape)} of "
+                  f"{lengths.dtype}")
+    tokens = torch.empty((batch, places), dtype=draft_tokens.dtype, device=target_probs.device)
+    accepted = torch.empty((batch,), dtype=torch.int32, device=target_probs.device)
+    if batch:
+        _call("pfa_verify_drafts", target_probs, draft_tokens.data_ptr(), size,
+              lengths.data_ptr() if lengths is not None else None, length_size, batch, drafts, vocab,
+              target_probs.data_ptr(), target_batch, target_place,
+              draft_probs.data_ptr() if draft_probs is not None else None, draft_batch, draft_place, kind,
+              uniforms.data_ptr(), noise.data_ptr(), noise.stride(0), tokens.data_ptr(), accepted.data_ptr(), None, 0)
+    return tokens, accepted

@@ -75,6 +75,12 @@ SIGNATURES = {
     "pfa_bsgs_apply_giants": (_i32, [_vp, _sz, _vp, C.POINTER(_vp), _sz, _sz, _vp, _sz, _vp, _vp]),
     "pfa_mod_raise": (_i32, [_vp, _vp, _sz, _vp, _vp]),
     "pfa_ct_lincomb": (_i32, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _vp, _vp, _vp]),
+    "pfa_quantize_int8": (_i32, [_vp, _sz, _i32, _sz, _sz, _vp, _sz, _vp, _vp]),
+    "pfa_rms_norm_int8": (_i32, [_vp, _sz, _vp, _sz, _vp, _i32, _sz, _sz, C.c_double, _vp, _sz, _vp, _sz, _vp, _vp]),
+    "pfa_int8_matmul": (_i32, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _i32, _sz, _vp, _sz, _vp]),
+    "pfa_token_probabilities": (_i32, [_vp, _sz, _i32, _sz, _sz, _vp, C.c_double, _vp, _sz, _vp, _vp, _sz, _vp]),
+    "pfa_verify_drafts": (_i32, [_vp, _i32, _vp, _i32, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _sz, _i32, _vp, _vp,
+                                 _sz, _vp, _vp, _vp, _sz, _vp]),
 }
 
 

@@ -18,6 +18,10 @@ generator and uploaded; the reference samples on the GPU with salsa20
 (src/prng.cu), whose streams are not reproducible anyway (seeds come from
 std::random_device).  Errors follow the reference's centred binomial
 distribution with 21 + 21 coin flips (sigma ~ 3.24, src/prng.cu:222-243).
+
+The clear end of an encrypted generation step (`quantize_int8`,
+`rms_norm_int8`, `int8_matmul`, `token_probabilities`, `verify_drafts`) works
+on plain torch tensors; clear_ops.py holds it.
 """
 from __future__ import annotations
 
@@ -31,6 +35,18 @@ import numpy as np
 import pfa_native as _N
 
 __version__ = "amd-1"
+
+_CLEAR_OPS = ("quantize_int8", "rms_norm_int8", "int8_matmul", "token_probabilities", "verify_drafts")
+
+
+def __getattr__(name):
+    """The operators of clear_ops, imported with torch on first use."""
+    if name in _CLEAR_OPS:
+        import clear_ops
+
+        f = globals()[name] = getattr(clear_ops, name)
+        return f
+    raise AttributeError(f"module 'pyPhantom' has no attribute {name!r}")
 
 _seed_counter = itertools.count()
 _global_seed = None
