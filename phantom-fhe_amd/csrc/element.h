@@ -24,6 +24,43 @@ void with_type(int type, F &&f) {
     fail(PFA_ERR_INVALID_ARGUMENT, "unknown element type " + std::to_string(type));
 }
 
+// V neighbouring elements as floats, from any address that is aligned to one element.
+// The words between are vector types: a plain array would be taken apart into
+// accesses of one element, while the memory takes 16 bytes at any alignment.
+template <int BYTES>
+struct WordsOf {
+    using type = uint32_t __attribute__((ext_vector_type(BYTES / 4)));
+};
+template <int V, class T>
+struct Elements {
+    T e[V];
+};
+template <int V, class T>
+__device__ __forceinline__ void load_vec(const T *p, float (&v)[V]) {
+    constexpr int kPart = sizeof(T) * V > 16 ? 16 : sizeof(T) * V, kEach = kPart / sizeof(T);
+#pragma unroll
+    for (int h = 0; h < V; h += kEach) {
+        typename WordsOf<kPart>::type w;
+        __builtin_memcpy(&w, p + h, kPart);
+        using Part = Elements<kEach, T>;
+        const auto t = __builtin_bit_cast(Part, w);
+#pragma unroll
+        for (int i = 0; i < kEach; i++) v[h + i] = (float)t.e[i];
+    }
+}
+template <int V, class T>
+__device__ __forceinline__ void store_vec(T *p, const float (&v)[V]) {
+    constexpr int kPart = sizeof(T) * V > 16 ? 16 : sizeof(T) * V, kEach = kPart / sizeof(T);
+#pragma unroll
+    for (int h = 0; h < V; h += kEach) {
+        Elements<kEach, T> t;
+#pragma unroll
+        for (int i = 0; i < kEach; i++) t.e[i] = (T)v[h + i];
+        using Words = typename WordsOf<kPart>::type;
+        const auto w = __builtin_bit_cast(Words, t);
+        __builtin_memcpy(p + h, &w, kPart);
+    }
+}
 inline size_t type_bytes(int type) {
     require(type == PFA_F32 || type == PFA_BF16 || type == PFA_F16, "unknown element type " + std::to_string(type));
     return type == PFA_F32 ? 4 : 2;

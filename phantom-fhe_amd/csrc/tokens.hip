@@ -30,42 +30,132 @@ struct RowStat {
     uint32_t top;  // largest |y w|, as mag_bits
 };
 
+struct RowArgs {
+    const void *x, *residual, *weight;
+    void *total;
+    int8_t *codes;
+    float *scales;
+    size_t rows, x_stride, residual_stride, total_stride, codes_stride;
+    uint32_t width;
+    float eps;
+};
+
+constexpr int kVec = 8;  // elements a thread takes at once: 16 bytes of the 2-byte types, 8 codes
+
+// v = (x + residual) weight of kVec places from i on (quantization: x itself), total and
+// the statistics on the way.  Places before `own` belong to another thread.
 template <class T, bool NORM>
-__global__ void __launch_bounds__(kRowThreads)
-k_quantize_rows(size_t rows, const T *x, size_t x_stride, const T *residual, size_t residual_stride, const T *weight,
-                uint32_t width, float eps, T *total, size_t total_stride, int8_t *codes, size_t codes_stride,
-                float *scales) {
-    __shared__ float part_sum[kRowThreads / 64];
-    __shared__ uint32_t part_top[kRowThreads / 64];
-    const size_t row = row_of();
-    if (row >= rows) return;
-    x += row * x_stride;
-    codes += row * codes_stride;
-    if (NORM && residual) {
-        residual += row * residual_stride;
-        total += row * total_stride;
-    }
-    RowStat s{0.f, 0u};
-    for (uint32_t i = threadIdx.x; i < width; i += kRowThreads) {
-        float v = (float)x[i];
-        if (NORM) {
-            if (residual) v += (float)residual[i];
-            s.sum = fmaf(v, v, s.sum);
-            v *= (float)weight[i];
+__device__ __forceinline__ void row_values(const RowArgs &a, const T *x, const T *residual, T *total, uint32_t i,
+                                           uint32_t own, RowStat &s, float (&v)[kVec]) {
+    load_vec<kVec>(x + i, v);
+    if (NORM) {
+        float w[kVec];
+        if (residual) {
+            load_vec<kVec>(residual + i, w);
+#pragma unroll
+            for (int e = 0; e < kVec; e++) v[e] += w[e];
+            if (total && own < a.width) store_vec<kVec>(total + i, v);
         }
-        s.top = max(s.top, mag_bits(v));
+        load_vec<kVec>(static_cast<const T *>(a.weight) + i, w);
+#pragma unroll
+        for (int e = 0; e < kVec; e++) {
+            const float y = i + e >= own ? v[e] : 0.f;
+            s.sum = fmaf(y, y, s.sum);
+            v[e] *= w[e];
+        }
     }
-    s.sum = wave_sum(s.sum);
+#pragma unroll
+    for (int e = 0; e < kVec; e++) s.top = max(s.top, mag_bits(v[e]));
+}
+
+// rows of fewer than kVec places
+template <class T, bool NORM>
+__device__ __forceinline__ void short_row_values(const RowArgs &a, const T *x, const T *residual, T *total,
+                                                 RowStat &s, float (&v)[kVec]) {
+#pragma unroll
+    for (int e = 0; e < kVec; e++) {
+        v[e] = 0.f;
+        if (e < (int)a.width) {
+            v[e] = (float)x[e];
+            if (NORM) {
+                if (residual) {
+                    v[e] += (float)residual[e];
+                    total[e] = (T)v[e];
+                }
+                s.sum = fmaf(v[e], v[e], s.sum);
+                v[e] *= (float)static_cast<const T *>(a.weight)[e];
+            }
+            s.top = max(s.top, mag_bits(v[e]));
+        }
+    }
+}
+
+// rint(v lift k) by one fused step: 1.5 2^23 leaves the sum's last bit at 1, so its low
+// byte is the code, rounded once to nearest even.  keep: ~0, or 0 for codes of 0.
+__device__ __forceinline__ uint32_t code_of(float v, float lift, float k) {
+    return __float_as_uint(fmaf(v * lift, k, 12582912.f));
+}
+__device__ __forceinline__ void store_codes(int8_t *codes, const float (&v)[kVec], float lift, float k, uint32_t keep) {
+    uint32_t w[kVec / 4];
+#pragma unroll
+    for (int e = 0; e < kVec; e += 4) {
+        const uint32_t lo = __builtin_amdgcn_perm(code_of(v[e + 1], lift, k), code_of(v[e], lift, k), 0x0c0c0400);
+        const uint32_t hi = __builtin_amdgcn_perm(code_of(v[e + 3], lift, k), code_of(v[e + 2], lift, k), 0x04000c0c);
+        w[e / 4] = (lo | hi) & keep;
+    }
+    __builtin_memcpy(codes, w, kVec);
+}
+
+// A row is read once: its values stay in registers, STEPS x kVec a thread, between the
+// reduction and the codes.  The row's last kVec places are one thread's even where the
+// width is no multiple of kVec (its vector then starts early, and threads past the end
+// read it too), so no load stands behind a branch and all of them are in flight at once.
+// THREADS = 64: four rows a workgroup, one a wave, no barrier.  STEPS = 0: rows too
+// long for the registers are read twice.
+template <class T, bool NORM, int THREADS, int STEPS>
+__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
+k_quantize_rows(RowArgs a) {
+    constexpr bool kWave = THREADS == 64;
+    constexpr int kHold = STEPS ? STEPS : 1;
+    const uint32_t t = threadIdx.x % THREADS;
+    const size_t row = kWave ? row_of() * 4 + threadIdx.x / 64 : row_of();
+    if (row >= a.rows) return;
+    const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+    const T *residual = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
+    T *total = residual ? static_cast<T *>(a.total) + row * a.total_stride : nullptr;
+    int8_t *codes = a.codes + row * a.codes_stride;
+    const bool brief = kWave && a.width < kVec;
+    const uint32_t last = a.width - kVec;
+    float v[kHold][kVec];
+    RowStat s{0.f, 0u};
+    if (brief) {
+        if (t == 0) short_row_values<T, NORM>(a, x, residual, total, s, v[0]);
+    } else if (STEPS) {
+#pragma unroll
+        for (int j = 0; j < kHold; j++) {
+            const uint32_t own = (j * THREADS + t) * kVec;
+            row_values<T, NORM>(a, x, residual, total, min(own, last), own, s, v[j]);
+        }
+    } else {
+        for (uint32_t own = t * kVec; own < a.width; own += THREADS * kVec)
+            row_values<T, NORM>(a, x, residual, total, min(own, last), own, s, v[0]);
+    }
+    s.sum = NORM ? wave_sum(s.sum) : 0.f;
     s.top = wave_max(s.top);
-    if (threadIdx.x % 64 == 0) {
-        part_sum[threadIdx.x / 64] = s.sum;
-        part_top[threadIdx.x / 64] = s.top;
-    }
-    __syncthreads();
-    s = {0.f, 0u};
-    for (int w = 0; w < kRowThreads / 64; w++) {
-        s.sum += part_sum[w];
-        s.top = max(s.top, part_top[w]);
+    if (!kWave) {
+        __shared__ float part_sum[THREADS / 64];
+        __shared__ uint32_t part_top[THREADS / 64];
+        if (t % 64 == 0) {
+            part_sum[t / 64] = s.sum;
+            part_top[t / 64] = s.top;
+        }
+        __syncthreads();
+        s = {0.f, 0u};
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; w++) {
+            s.sum += part_sum[w];
+            s.top = max(s.top, part_top[w]);
+        }
     }
     // a NaN, an infinity or a sum past float's range: a NaN scale, codes of 0
     const bool bad = s.top >= kInfBits || !(s.sum < __uint_as_float(kInfBits));
@@ -75,23 +165,52 @@ k_quantize_rows(size_t rows, const T *x, size_t x_stride, const T *residual, siz
         lift = 0x1p64f;
         top *= lift;
     }
-    const float k = bad || s.top == 0 ? 0.f : 127.f / top;
-    if (threadIdx.x == 0) {
+    const float k = s.top == 0 ? 0.f : 127.f / top;
+    const uint32_t keep = bad ? 0u : ~0u;
+    if (t == 0) {
         float scale = __uint_as_float(s.top) / 127.f;
-        if (NORM) scale *= rsqrtf(s.sum / (float)width + eps);
-        scales[row] = bad ? __uint_as_float(0x7fc00000u) : scale;
+        if (NORM) scale *= rsqrtf(s.sum / (float)a.width + a.eps);
+        a.scales[row] = bad ? __uint_as_float(0x7fc00000u) : scale;
     }
-    for (uint32_t i = threadIdx.x; i < width; i += kRowThreads) {
-        float v = (float)x[i];
-        if (NORM) {
-            if (residual) {
-                v += (float)residual[i];
-                total[i] = (T)v;
-            }
-            v *= (float)weight[i];
+    if (brief) {
+        if (t == 0)
+#pragma unroll
+            for (int e = 0; e < kVec; e++)
+                if (e < (int)a.width) codes[e] = (int8_t)(code_of(v[0][e], lift, k) & keep);
+    } else if (STEPS) {
+#pragma unroll
+        for (int j = 0; j < kHold; j++) {
+            const uint32_t own = (j * THREADS + t) * kVec;
+            if (own < a.width) store_codes(codes + min(own, last), v[j], lift, k, keep);
         }
-        codes[i] = bad ? 0 : (int8_t)(int)rintf(v * lift * k);
+    } else {
+        RowStat again{0.f, 0u};
+        for (uint32_t own = t * kVec; own < a.width; own += THREADS * kVec) {
+            row_values<T, NORM>(a, x, residual, nullptr, min(own, last), own, again, v[0]);
+            store_codes(codes + min(own, last), v[0], lift, k, keep);
+        }
     }
+}
+
+template <class T, bool NORM, int THREADS, int STEPS>
+void launch_rows(const RowArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((k_quantize_rows<T, NORM, THREADS, STEPS>),
+                       row_grid(THREADS == 64 ? (a.rows + 3) / 4 : a.rows), dim3(THREADS < 256 ? 256 : THREADS), 0, s,
+                       a);
+}
+
+template <class T, bool NORM>
+void quantize_rows(const RowArgs &a, hipStream_t s) {
+    const uint32_t vecs = (a.width + kVec - 1) / kVec;
+    if (vecs <= 64) return launch_rows<T, NORM, 64, 1>(a, s);
+    if (vecs <= 256) return launch_rows<T, NORM, 256, 1>(a, s);
+    if (vecs <= 512) return launch_rows<T, NORM, 256, 2>(a, s);
+    if (vecs <= 1024) return launch_rows<T, NORM, 256, 4>(a, s);
+    if (vecs <= 2048) return launch_rows<T, NORM, 256, 8>(a, s);
+    if (vecs <= 4096) return launch_rows<T, NORM, 1024, 4>(a, s);
+    // the norm's three inputs of 8 steps would pass 128 registers, 1024 threads' share
+    if (!NORM && vecs <= 8192) return launch_rows<T, NORM, 1024, NORM ? 0 : 8>(a, s);
+    launch_rows<T, NORM, 1024, 0>(a, s);
 }
 
 // Probabilities of one row: exp2((l - m) c) / sum, c = log2(e) / temperature, m the
@@ -275,13 +394,15 @@ int pfa_quantize_int8(const void *x, size_t x_stride, int type, size_t rows, siz
         require(apart(rows, x_stride, width) && apart(rows, codes_stride, width, true), "rows overlap");
         aligned(x, size, "x");
         aligned(scales, 4, "scales");
-        with_type(type, [&](auto t) {
-            using T = decltype(t);
-            hipLaunchKernelGGL((k_quantize_rows<T, false>), row_grid(rows), dim3(kRowThreads), 0,
-                               as_stream(stream), rows, (const T *)x, x_stride, (const T *)nullptr, (size_t)0,
-                               (const T *)nullptr, (uint32_t)width, 0.f, (T *)nullptr, (size_t)0, codes, codes_stride,
-                               scales);
-        });
+        RowArgs a{};
+        a.x = x;
+        a.codes = codes;
+        a.scales = scales;
+        a.rows = rows;
+        a.x_stride = x_stride;
+        a.codes_stride = codes_stride;
+        a.width = (uint32_t)width;
+        with_type(type, [&](auto t) { quantize_rows<decltype(t), false>(a, as_stream(stream)); });
         PFA_HIP(hipGetLastError());
     });
 }
@@ -305,13 +426,9 @@ int pfa_rms_norm_int8(const void *x, size_t x_stride, const void *residual, size
         aligned(weight, size, "weight");
         aligned(total, size, "total");
         aligned(scales, 4, "scales");
-        with_type(type, [&](auto t) {
-            using T = decltype(t);
-            hipLaunchKernelGGL((k_quantize_rows<T, true>), row_grid(rows), dim3(kRowThreads), 0,
-                               as_stream(stream), rows, (const T *)x, x_stride, (const T *)residual, residual_stride,
-                               (const T *)weight, (uint32_t)width, (float)eps, (T *)total, total_stride, codes,
-                               codes_stride, scales);
-        });
+        const RowArgs a{x,        residual,        weight,       total,        codes,           scales, rows,
+                        x_stride, residual_stride, total_stride, codes_stride, (uint32_t)width, (float)eps};
+        with_type(type, [&](auto t) { quantize_rows<decltype(t), true>(a, as_stream(stream)); });
         PFA_HIP(hipGetLastError());
     });
 }
