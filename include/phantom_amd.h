@@ -431,6 +431,10 @@ int pfa_int8_matmul(const int8_t *a, size_t a_stride, const float *a_scales, con
                     const float *b_scales, const float *bias, size_t M, size_t N, size_t K, void *out, int type,
                     size_t out_stride, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Bytes of workspace that pfa_token_probabilities (rows x vocab) and
+ * pfa_verify_drafts (rows = batch) need at most. */
+int pfa_token_workspace(size_t rows, size_t vocab, size_t *bytes);
+
 /* Probabilities out [rows][vocab] of logits [rows][vocab]: softmax(logits /
  * temperature) over the places where mask [rows][vocab] (bytes; mask_stride 0:
  * one row for all; NULL: everywhere) is not 0; 0 elsewhere, whatever stands
@@ -438,7 +442,8 @@ int pfa_int8_matmul(const int8_t *a, size_t a_stride, const float *a_scales, con
  * temperatures is NULL; at 0 the lowest place of the largest logit gets 1.  A row
  * that allows nothing, or -infinity alone, is all 0.  A NaN or (above temperature
  * 0) +infinity in an allowed place, or a negative or NaN temperature, makes the
- * row's allowed places NaN.  workspace as in pfa_int8_matmul. */
+ * row's allowed places NaN.  workspace: pfa_token_workspace bytes, otherwise as in
+ * pfa_int8_matmul. */
 int pfa_token_probabilities(const void *logits, size_t stride, int type, size_t rows, size_t vocab,
                             const float *temperatures, double temperature, const uint8_t *mask, size_t mask_stride,
                             float *out, void *workspace, size_t workspace_bytes, void *stream);
@@ -456,8 +461,8 @@ int pfa_token_probabilities(const void *logits, size_t stride, int type, size_t 
  * token drawn, then -1; accepted [batch]: n.  Tokens have token_bytes (4 or 8),
  * lengths length_bytes.  uniforms [batch][K]; the strides are of target and draft
  * (from sequence to sequence, from place to place) and of noise.  All arithmetic
- * is in 32-bit floats, each operation rounded once.  workspace as in
- * pfa_int8_matmul. */
+ * is in 32-bit floats, each operation rounded once.  workspace: pfa_token_workspace
+ * bytes, otherwise as in pfa_int8_matmul. */
 int pfa_verify_drafts(const void *drafts, int token_bytes, const void *lengths, int length_bytes, size_t batch,
                       size_t K, size_t vocab, const void *target, size_t target_batch, size_t target_place,
                       const void *draft, size_t draft_batch, size_t draft_place, int type, const float *uniforms,

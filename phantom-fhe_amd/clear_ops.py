@@ -80,6 +80,15 @@ def _new_codes(shape, device):
     return torch.empty((*shape[:-1], -(-width // 16) * 16), dtype=torch.int8, device=device)[..., :width]
 
 
+def _workspace(rows, vocab, device):
+    """(tensor to hold on to, address, bytes) of the workspace of a row of places for each of rows."""
+    need = _N.token_workspace(rows, vocab)
+    if not need:
+        return None, None, 0
+    t = torch.empty((need,), dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), need
+
+
 def quantize_int8(x):
     """Codes of 8 bits of x [..., width], with one scale for each row: (codes int8
     [..., width], scales float32 [...]), x ~ codes * scales.
@@ -203,9 +212,10 @@ def token_probabilities(logits, temperature=1.0, mask=None):
     _same_device(logits, temperature=temperatures, mask=mask)
     out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
     if out.numel():
+        held, space, size = _workspace(n, vocab, out.device)
         _call("pfa_token_probabilities", logits, rows.data_ptr(), stride, kind, n, vocab,
               temperatures.data_ptr() if temperatures is not None else None, one,
-              allowed.data_ptr() if allowed is not None else None, mask_stride, out.data_ptr(), None, 0)
+              allowed.data_ptr() if allowed is not None else None, mask_stride, out.data_ptr(), space, size)
     return out
 
 
@@ -268,9 +278,11 @@ def verify_drafts(draft_tokens, target_probs, uniforms, noise, draft_probs=None,
     tokens = torch.empty((batch, places), dtype=draft_tokens.dtype, device=target_probs.device)
     accepted = torch.empty((batch,), dtype=torch.int32, device=target_probs.device)
     if batch:
+        held, space, need = _workspace(batch, vocab, tokens.device)
         _call("pfa_verify_drafts", target_probs, draft_tokens.data_ptr(), size,
               lengths.data_ptr() if lengths is not None else None, length_size, batch, drafts, vocab,
               target_probs.data_ptr(), target_batch, target_place,
               draft_probs.data_ptr() if draft_probs is not None else None, draft_batch, draft_place, kind,
-              uniforms.data_ptr(), noise.data_ptr(), noise.stride(0), tokens.data_ptr(), accepted.data_ptr(), None, 0)
+              uniforms.data_ptr(), noise.data_ptr(), noise.stride(0), tokens.data_ptr(), accepted.data_ptr(), space,
+              need)
     return tokens, accepted

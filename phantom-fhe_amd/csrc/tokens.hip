@@ -215,63 +215,351 @@ void quantize_rows(const RowArgs &a, hipStream_t s) {
 
 // Probabilities of one row: exp2((l - m) c) / sum, c = log2(e) / temperature, m the
 // largest allowed logit; temperature 0 leaves the lowest place of m alone.
+struct ProbArgs {
+    const void *logits;
+    const float *temperatures;
+    const uint8_t *mask;
+    float *out;
+    void *parts;  // [rows][chunks] of ProbPart
+    size_t rows, stride, mask_stride;
+    uint32_t vocab, chunk, chunks;
+    float temperature;
+};
+
+constexpr float kLog2e = 1.44269504088896341f;
+__device__ __forceinline__ float infinity() { return __uint_as_float(kInfBits); }
+__device__ __forceinline__ float not_a_number() { return __uint_as_float(0x7fc00000u); }
+
+// log2(e) / t within float's range: a subnormal t must not make 0 c a NaN
+__device__ __forceinline__ float rate_of(float t) { return fminf(kLog2e / t, 3e38f); }
+
+// e^((l - m) / t).  The bound takes -infinity (also at an infinite t) to 0; m is finite.
+__device__ __forceinline__ float weight_of(float l, float m, float c) {
+    return __builtin_amdgcn_exp2f(fmaxf((l - m) * c, -200.f));
+}
+
+// kVec logits from i on, -infinity where no token is allowed or the place is before `own`
 template <class T>
-__global__ void __launch_bounds__(kRowThreads)
-k_probabilities(size_t rows, const T *logits, size_t stride, const float *temperatures, float temperature, const uint8_t *mask,
-                size_t mask_stride, uint32_t vocab, float *out) {
-    __shared__ float part[kRowThreads / 64];
-    __shared__ uint32_t first;
-    const size_t row = row_of();
-    if (row >= rows) return;
-    logits += row * stride;
-    out += row * vocab;
-    if (mask) mask += row * mask_stride;
-    const float inf = __uint_as_float(kInfBits);
-    const float t = temperatures ? temperatures[row] : temperature;
-    const float c = fminf(1.44269504088896341f / t, 3e38f);
-    float m = -inf;
-    bool nan = !(t >= 0.f);
-    for (uint32_t i = threadIdx.x; i < vocab; i += kRowThreads) {
-        if (mask && !mask[i]) continue;
-        const float l = (float)logits[i];
-        nan |= l != l;
-        m = fmaxf(m, l);
+__device__ __forceinline__ void allowed_logits(const T *logits, const uint8_t *mask, uint32_t i, uint32_t own,
+                                               float (&v)[kVec]) {
+    load_vec<kVec>(logits + i, v);
+    if (mask) {
+        const uint8_t *p = mask + i;
+        uint32_t w[2];
+        __builtin_memcpy(w, p, 8);
+#pragma unroll
+        for (int e = 0; e < kVec; e++) v[e] = (w[e / 4] >> (e % 4 * 8) & 0xff) ? v[e] : -infinity();
     }
-    m = wave_max(nan ? inf : m);
-    if (threadIdx.x == 0) first = 0xffffffffu;
-    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = m;
-    nan = __syncthreads_or(nan);
-    m = part[0];
-    for (int w = 1; w < kRowThreads / 64; w++) m = fmaxf(m, part[w]);
-    __syncthreads();
-    if (t == 0.f) {
-        for (uint32_t i = threadIdx.x; i < vocab; i += kRowThreads)
-            if ((!mask || mask[i]) && (float)logits[i] == m && m > -inf) {
-                atomicMin(&first, i);
-                break;
+#pragma unroll
+    for (int e = 0; e < kVec; e++) v[e] = i + e >= own ? v[e] : -infinity();
+}
+
+// What a stretch of a row says: its largest logit, the sum of weights against it, the
+// lowest place of the largest.  A NaN in an allowed place is a NaN sum.
+struct __align__(16) ProbPart {
+    float top, sum;
+    uint32_t first, unused;
+};
+
+// A row, or a stretch of one, by THREADS threads: values stay in registers.
+template <class T, int THREADS, int STEPS>
+struct ProbRow {
+    float v[STEPS][kVec];
+    float top = -infinity();
+    bool nan = false;
+
+    __device__ __forceinline__ void load(const T *logits, const uint8_t *mask, uint32_t begin, uint32_t end) {
+        const uint32_t last = end - kVec;
+#pragma unroll
+        for (int j = 0; j < STEPS; j++) {
+            const uint32_t own = begin + (j * THREADS + threadIdx.x) * kVec;
+            allowed_logits(logits, mask, min(own, last), own, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < STEPS; j++)
+#pragma unroll
+            for (int e = 0; e < kVec; e++) {
+                nan |= v[j][e] != v[j][e];
+                top = fmaxf(top, v[j][e]);
             }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < vocab; i += kRowThreads)
-            out[i] = nan ? (!mask || mask[i] ? __uint_as_float(0x7fc00000u) : 0.f) : i == first ? 1.f : 0.f;
-        return;
     }
-    float sum = 0.f;
-    for (uint32_t i = threadIdx.x; i < vocab; i += kRowThreads) {
-        if (mask && !mask[i]) continue;
-        const float l = (float)logits[i];
-        if (l != -inf) sum += exp2f((l - m) * c);
+    // the largest of all threads; whether any saw a NaN
+    __device__ __forceinline__ void share_top() {
+        __shared__ float part[THREADS / 64];
+        const float w = wave_max(top);
+        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = w;
+        nan = __syncthreads_or(nan);
+        top = part[0];
+#pragma unroll
+        for (int i = 1; i < THREADS / 64; i++) top = fmaxf(top, part[i]);
+    }
+    // values become weights against `m`; their sum over all threads
+    __device__ __forceinline__ float weights(float m, float c) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < STEPS; j++)
+#pragma unroll
+            for (int e = 0; e < kVec; e++) {
+                v[j][e] = weight_of(v[j][e], m, c);
+                sum += v[j][e];
+            }
+        __shared__ float part[THREADS / 64];
+        sum = wave_sum(sum);
+        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = sum;
+        __syncthreads();
+        sum = part[0];
+#pragma unroll
+        for (int i = 1; i < THREADS / 64; i++) sum += part[i];
+        return sum;
+    }
+    // lowest place of `m`
+    __device__ __forceinline__ uint32_t first(float m, uint32_t begin, uint32_t end) {
+        __shared__ uint32_t at;
+        if (threadIdx.x == 0) at = 0xffffffffu;
+        __syncthreads();
+        const uint32_t last = end - kVec;
+        uint32_t low = 0xffffffffu;
+#pragma unroll
+        for (int j = 0; j < STEPS; j++) {
+            const uint32_t i = min(begin + (j * THREADS + (uint32_t)threadIdx.x) * kVec, last);
+#pragma unroll
+            for (int e = 0; e < kVec; e++)
+                if (v[j][e] == m) low = min(low, i + e);
+        }
+        if (low != 0xffffffffu) atomicMin(&at, low);
+        __syncthreads();
+        return at;
+    }
+};
+
+// A row of NaN: its allowed places, 0 elsewhere.
+__device__ __forceinline__ void write_nan(const uint8_t *mask, float *out, uint32_t begin, uint32_t end,
+                                          uint32_t threads) {
+    for (uint32_t i = begin + threadIdx.x; i < end; i += threads) out[i] = !mask || mask[i] ? not_a_number() : 0.f;
+}
+
+// Rows in one piece: read once, reduced twice, written once.
+template <class T, int THREADS, int STEPS>
+__global__ void __launch_bounds__(THREADS)
+k_prob_rows(ProbArgs a) {
+    const size_t row = row_of();
+    if (row >= a.rows) return;
+    const T *logits = static_cast<const T *>(a.logits) + row * a.stride;
+    const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
+    float *out = a.out + row * a.vocab;
+    const float t = a.temperatures ? a.temperatures[row] : a.temperature;
+    ProbRow<T, THREADS, STEPS> r;
+    r.load(logits, mask, 0, a.vocab);
+    r.share_top();
+    if (r.nan || !(t >= 0.f) || (t > 0.f && r.top == infinity()))
+        return write_nan(mask, out, 0, a.vocab, THREADS);
+    const bool greedy = t == 0.f;
+    const uint32_t at = greedy && r.top > -infinity() ? r.first(r.top, 0, a.vocab) : 0xffffffffu;
+    const float sum = r.weights(r.top == -infinity() ? 0.f : r.top, rate_of(t));
+    const float scale = sum > 0.f ? 1.f / sum : 0.f;
+    const uint32_t last = a.vocab - kVec;
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) {
+        const uint32_t own = (j * THREADS + threadIdx.x) * kVec, i = min(own, last);
+#pragma unroll
+        for (int e = 0; e < kVec; e++) r.v[j][e] = greedy ? (i + e == at ? 1.f : 0.f) : r.v[j][e] * scale;
+        // a place before `own` holds weight 0 here and its probability elsewhere
+        if (i == own) {
+            store_vec<kVec>(out + i, r.v[j]);
+        } else if (own < a.vocab) {
+#pragma unroll
+            for (int e = 0; e < kVec; e++)
+                if (i + e >= own) out[i + e] = r.v[j][e];
+        }
+    }
+}
+
+// Long rows, and few rows: stretches of `chunk` places by a workgroup each, in two
+// launches.  The first leaves a ProbPart for each stretch, the second joins a row's and
+// writes the probabilities; its second reading of the logits comes from the caches.
+constexpr int kChunkThreads = 256;
+
+template <class T, int STEPS>
+__global__ void __launch_bounds__(kChunkThreads)
+k_prob_parts(ProbArgs a) {
+    const size_t job = row_of(), row = job / a.chunks;
+    if (row >= a.rows) return;
+    const uint32_t begin = (uint32_t)(job % a.chunks) * a.chunk, end = min(begin + a.chunk, a.vocab);
+    const T *logits = static_cast<const T *>(a.logits) + row * a.stride;
+    const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
+    const float t = a.temperatures ? a.temperatures[row] : a.temperature;
+    ProbRow<T, kChunkThreads, STEPS> r;
+    r.load(logits, mask, begin, end);
+    r.share_top();
+    ProbPart p{r.top, 0.f, 0xffffffffu, 0u};
+    if (r.nan || !(t >= 0.f) || (t > 0.f && r.top == infinity()))
+        p.sum = not_a_number();
+    else if (t == 0.f)
+        p.first = r.top == -infinity() ? 0xffffffffu : r.first(r.top, begin, end);
+    else
+        p.sum = r.weights(r.top == -infinity() ? 0.f : r.top, rate_of(t));
+    if (threadIdx.x == 0) static_cast<ProbPart *>(a.parts)[job] = p;
+}
+
+template <class T, int STEPS>
+__global__ void __launch_bounds__(kChunkThreads)
+k_prob_write(ProbArgs a) {
+    __shared__ float part[kChunkThreads / 64], part_sum[kChunkThreads / 64];
+    __shared__ uint32_t part_first[kChunkThreads / 64];
+    const size_t job = row_of(), row = job / a.chunks;
+    if (row >= a.rows) return;
+    const uint32_t begin = (uint32_t)(job % a.chunks) * a.chunk, end = min(begin + a.chunk, a.vocab);
+    const uint32_t last = end - kVec, wave = threadIdx.x / 64;
+    const T *logits = static_cast<const T *>(a.logits) + row * a.stride;
+    const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
+    float *out = a.out + row * a.vocab;
+    const float t = a.temperatures ? a.temperatures[row] : a.temperature;
+    const float c = rate_of(t);
+    float v[STEPS][kVec];
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) {
+        const uint32_t own = begin + (j * kChunkThreads + threadIdx.x) * kVec;
+        allowed_logits(logits, mask, min(own, last), 0, v[j]);
+    }
+    const ProbPart *parts = static_cast<const ProbPart *>(a.parts) + row * a.chunks;
+    float top = -infinity(), sum = 0.f;
+    uint32_t first = 0xffffffffu;
+    for (uint32_t i = threadIdx.x; i < a.chunks; i += kChunkThreads) top = fmaxf(top, parts[i].top);
+    top = wave_max(top);
+    if (threadIdx.x % 64 == 0) part[wave] = top;
+    __syncthreads();
+    top = part[0];
+#pragma unroll
+    for (int i = 1; i < kChunkThreads / 64; i++) top = fmaxf(top, part[i]);
+    const float m = top == -infinity() ? 0.f : top;
+    for (uint32_t i = threadIdx.x; i < a.chunks; i += kChunkThreads) {
+        const ProbPart p = parts[i];
+        if (t == 0.f && p.top == top) first = min(first, p.first);
+        sum += t == 0.f ? p.sum : p.sum == 0.f ? 0.f : p.sum * weight_of(p.top, m, c);
     }
     sum = wave_sum(sum);
-    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = sum;
+    first = ~wave_max(~first);
+    if (threadIdx.x % 64 == 0) {
+        part_sum[wave] = sum;
+        part_first[wave] = first;
+    }
     __syncthreads();
     sum = 0.f;
-    for (int w = 0; w < kRowThreads / 64; w++) sum += part[w];
-    const float scale = nan ? __uint_as_float(0x7fc00000u) : m == -inf ? 0.f : 1.f / sum;
-    for (uint32_t i = threadIdx.x; i < vocab; i += kRowThreads) {
-        const float l = (float)logits[i];
-        const bool in = !mask || mask[i];
-        out[i] = !in ? 0.f : l == -inf ? 0.f * scale : exp2f((l - m) * c) * scale;
+    first = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < kChunkThreads / 64; i++) {
+        sum += part_sum[i];
+        first = min(first, part_first[i]);
     }
+    if (sum != sum) return write_nan(mask, out, begin, end, kChunkThreads);
+    const float scale = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) {
+        const uint32_t own = begin + (j * kChunkThreads + threadIdx.x) * kVec, i = min(own, last);
+#pragma unroll
+        for (int e = 0; e < kVec; e++)
+            v[j][e] = t == 0.f ? (i + e == first ? 1.f : 0.f) : weight_of(v[j][e], m, c) * scale;
+        if (own < end) store_vec<kVec>(out + i, v[j]);
+    }
+}
+
+// rows of fewer than kVec places, one a thread
+template <class T>
+__global__ void __launch_bounds__(kRowThreads)
+k_prob_short(ProbArgs a) {
+    const size_t row = row_of() * kRowThreads + threadIdx.x;
+    if (row >= a.rows) return;
+    const T *logits = static_cast<const T *>(a.logits) + row * a.stride;
+    const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
+    float *out = a.out + row * a.vocab;
+    const float t = a.temperatures ? a.temperatures[row] : a.temperature;
+    float top = -infinity(), sum = 0.f;
+    uint32_t first = 0xffffffffu;
+    bool nan = !(t >= 0.f);
+    for (uint32_t i = 0; i < a.vocab; i++) {
+        const float l = !mask || mask[i] ? (float)logits[i] : -infinity();
+        nan |= l != l;
+        if (l > top) {
+            top = l;
+            first = i;
+        }
+    }
+    if (nan || (t > 0.f && top == infinity())) {
+        for (uint32_t i = 0; i < a.vocab; i++) out[i] = !mask || mask[i] ? not_a_number() : 0.f;
+        return;
+    }
+    const float c = rate_of(t), m = top == -infinity() ? 0.f : top;
+    for (int write = 0; write < 2; write++) {
+        const float scale = sum > 0.f ? 1.f / sum : 0.f;
+        for (uint32_t i = 0; i < a.vocab; i++) {
+            const float l = !mask || mask[i] ? (float)logits[i] : -infinity();
+            const float w = t == 0.f ? (i == first ? 1.f : 0.f) : weight_of(l, m, c);
+            if (write)
+                out[i] = w * scale;
+            else
+                sum += w;
+        }
+    }
+}
+
+// How a call is cut: chunks == 1 is one workgroup a row.
+struct Cut {
+    uint32_t chunk, chunks;
+};
+Cut cut_probabilities(size_t rows, uint32_t vocab) {
+    if (vocab < kVec) return {vocab, 1};
+    // one piece: up to 64 values a thread stay in registers.  Few long rows leave most of
+    // the card idle so, and are cut.
+    if (vocab <= 65536 && (rows >= 128 || vocab <= 8192)) return {vocab, 1};
+    uint32_t steps = 8;
+    while (steps > 1 && rows * ((vocab + steps * kChunkThreads * kVec - 1) / (steps * kChunkThreads * kVec)) < 1024)
+        steps /= 2;
+    const uint32_t chunk = steps * kChunkThreads * kVec;
+    return {chunk, (vocab + chunk - 1) / chunk};
+}
+
+template <class T>
+void probabilities(const ProbArgs &a, hipStream_t s) {
+    const uint32_t vecs = (a.vocab + kVec - 1) / kVec;
+#define PFA_LAUNCH(kernel, jobs, threads) hipLaunchKernelGGL((kernel), row_grid(jobs), dim3(threads), 0, s, a)
+    if (a.vocab < kVec) {
+        PFA_LAUNCH(k_prob_short<T>, (a.rows + kRowThreads - 1) / kRowThreads, kRowThreads);
+    } else if (a.chunks == 1) {
+        if (vecs <= 64)
+            PFA_LAUNCH((k_prob_rows<T, 64, 1>), a.rows, 64);
+        else if (vecs <= 256)
+            PFA_LAUNCH((k_prob_rows<T, 256, 1>), a.rows, 256);
+        else if (vecs <= 512)
+            PFA_LAUNCH((k_prob_rows<T, 256, 2>), a.rows, 256);
+        else if (vecs <= 1024)
+            PFA_LAUNCH((k_prob_rows<T, 256, 4>), a.rows, 256);
+        else if (vecs <= 2048)
+            PFA_LAUNCH((k_prob_rows<T, 256, 8>), a.rows, 256);
+        else if (vecs <= 4096)
+            PFA_LAUNCH((k_prob_rows<T, 1024, 4>), a.rows, 1024);
+        else
+            PFA_LAUNCH((k_prob_rows<T, 1024, 8>), a.rows, 1024);
+    } else {
+        const size_t jobs = a.rows * a.chunks;
+        switch (a.chunk / (kChunkThreads * kVec)) {
+            case 1:
+                PFA_LAUNCH((k_prob_parts<T, 1>), jobs, kChunkThreads);
+                PFA_LAUNCH((k_prob_write<T, 1>), jobs, kChunkThreads);
+                break;
+            case 2:
+                PFA_LAUNCH((k_prob_parts<T, 2>), jobs, kChunkThreads);
+                PFA_LAUNCH((k_prob_write<T, 2>), jobs, kChunkThreads);
+                break;
+            case 4:
+                PFA_LAUNCH((k_prob_parts<T, 4>), jobs, kChunkThreads);
+                PFA_LAUNCH((k_prob_write<T, 4>), jobs, kChunkThreads);
+                break;
+            default:
+                PFA_LAUNCH((k_prob_parts<T, 8>), jobs, kChunkThreads);
+                PFA_LAUNCH((k_prob_write<T, 8>), jobs, kChunkThreads);
+        }
+    }
+#undef PFA_LAUNCH
 }
 
 struct VerifyArgs {
@@ -283,9 +571,10 @@ struct VerifyArgs {
     const float *noise;     // [batch][vocab]
     void *tokens;           // [batch][K + 1], like drafts
     int32_t *accepted;      // [batch]
+    uint64_t *parts;        // [batch][chunks] race keys, with more than one chunk
     size_t target_batch, target_place, draft_batch, draft_place, noise_batch;  // strides in elements
     size_t batch;
-    uint32_t K, vocab;
+    uint32_t K, vocab, chunk, chunks;
     bool tokens64, lengths64;
 };
 
@@ -297,58 +586,89 @@ __device__ __forceinline__ int64_t whole(const void *p, size_t i, bool wide) {
 __device__ __forceinline__ uint64_t race_key(float w, float e, uint32_t i) {
     return w > 0.f ? (uint64_t)__float_as_uint(w / e) << 32 | (0xffffffffu - i) : 0;
 }
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-// One sequence a workgroup.  Draft i stays while u_i q_i(x_i) < p_i(x_i); the token
-// after the first that does not is drawn from max(p - q, 0), after the last one from
-// p: the largest weight / noise, an exponential race, has exactly that distribution.
-// Each product, difference and quotient is one rounding of 32 bits, so the choice
-// does not depend on the order of anything.
+__device__ __forceinline__ uint32_t length_of(const VerifyArgs &a, size_t b) {
+    const int64_t given = a.lengths ? whole(a.lengths, b, a.lengths64) : (int64_t)a.K;
+    return (uint32_t)(given < 0 ? 0 : given > (int64_t)a.K ? (int64_t)a.K : given);
+}
+
+// How many of the drafts of sequence b are kept: every wave looks at 64 of them at once,
+// so the two dependent readings (token, then probability) are paid once and not K times.
 template <class T>
-__global__ void __launch_bounds__(kRowThreads)
-k_verify(VerifyArgs a) {
+__device__ __forceinline__ uint32_t kept(const VerifyArgs &a, size_t b, uint32_t len) {
 #pragma clang fp contract(off)
-    __shared__ uint64_t best_rest[kRowThreads / 64], best_all[kRowThreads / 64];
-    const size_t b = row_of();
-    if (b >= a.batch) return;
     const T *target = static_cast<const T *>(a.target) + b * a.target_batch;
     const T *draft = static_cast<const T *>(a.draft) + b * a.draft_batch;
-    const int64_t given = a.lengths ? whole(a.lengths, b, a.lengths64) : (int64_t)a.K;
-    const uint32_t len = (uint32_t)(given < 0 ? 0 : given > (int64_t)a.K ? (int64_t)a.K : given);
-    uint32_t n = 0;
-    for (; n < len; n++) {
-        const int64_t x = whole(a.drafts, b * a.K + n, a.tokens64);
-        if (x < 0 || x >= (int64_t)a.vocab) break;
-        const float p = (float)target[n * a.target_place + x];
-        const float q = a.draft ? (float)draft[n * a.draft_place + x] : 1.f;
-        if (!(a.uniforms[b * a.K + n] * q < p)) break;
-    }
-    target += n * a.target_place;
-    const bool rest = n < len;
-    const int64_t refused = rest ? whole(a.drafts, b * a.K + n, a.tokens64) : -1;
-    const float *noise = a.noise + b * a.noise_batch;
-    uint64_t key_rest = 0, key_all = 0;
-    for (uint32_t i = threadIdx.x; i < a.vocab; i += kRowThreads) {
-        const float p = (float)target[i], e = noise[i];
-        const uint64_t k = race_key(p, e, i);
-        key_all = k > key_all ? k : key_all;
-        if (rest) {
-            const float w = a.draft ? p - (float)draft[n * a.draft_place + i] : (int64_t)i == refused ? 0.f : p;
-            const uint64_t r = race_key(w, e, i);
-            key_rest = r > key_rest ? r : key_rest;
+    for (uint32_t n = 0; n < len; n += 64) {
+        const uint32_t i = n + threadIdx.x % 64;
+        bool keep = false;
+        if (i < len) {
+            const int64_t x = whole(a.drafts, b * a.K + i, a.tokens64);
+            if (x >= 0 && x < (int64_t)a.vocab) {
+                const float p = (float)target[i * a.target_place + x];
+                const float q = a.draft ? (float)draft[i * a.draft_place + x] : 1.f;
+                keep = a.uniforms[b * a.K + i] * q < p;
+            }
         }
+        const uint64_t lost = ~__ballot(keep);
+        if (lost) return min(n + (uint32_t)__builtin_ctzll(lost), len);
     }
-    key_all = wave_max(key_all);
-    key_rest = wave_max(key_rest);
-    if (threadIdx.x % 64 == 0) {
-        best_all[threadIdx.x / 64] = key_all;
-        best_rest[threadIdx.x / 64] = key_rest;
+    return len;
+}
+
+constexpr uint32_t kNowhere = 0xffffffffu;
+
+// Largest key over the places [begin, end) of w / noise: w = target, less the draft's
+// where `draft` is given, but 0 at place `without`.
+template <class T>
+__device__ __forceinline__ uint64_t race(const T *target, const T *draft, const float *noise, uint32_t without,
+                                         uint32_t begin, uint32_t end, uint32_t threads) {
+#pragma clang fp contract(off)
+    uint64_t key = 0;
+    uint32_t i = begin + threadIdx.x * kVec;
+    for (; i + kVec <= end; i += threads * kVec) {
+        float e[kVec], w[kVec];
+        load_vec<kVec>(noise + i, e);
+        load_vec<kVec>(target + i, w);
+        if (draft) {
+            float q[kVec];
+            load_vec<kVec>(draft + i, q);
+#pragma unroll
+            for (int k = 0; k < kVec; k++) w[k] -= q[k];
+        }
+#pragma unroll
+        for (int k = 0; k < kVec; k++) key = larger(key, race_key(i + k == without ? 0.f : w[k], e[k], i + k));
     }
+    for (; i < end; i++) {
+        const float w = (float)target[i] - (draft ? (float)draft[i] : 0.f);
+        key = larger(key, race_key(i == without ? 0.f : w, noise[i], i));
+    }
+    return key;
+}
+
+template <int THREADS>
+__device__ __forceinline__ uint64_t block_largest(uint64_t key) {
+    __shared__ uint64_t part[THREADS / 64];
+    key = wave_max(key);
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = key;
     __syncthreads();
-    for (int w = 0; w < kRowThreads / 64; w++) {
-        key_all = best_all[w] > key_all ? best_all[w] : key_all;
-        key_rest = best_rest[w] > key_rest ? best_rest[w] : key_rest;
+    key = part[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; i++) key = larger(key, part[i]);
+    __syncthreads();
+    return key;
+}
+
+// The tokens of sequence b, given the winner of its race.  A refusal that leaves nothing
+// over is rare: the target's own race is run here then.
+template <class T>
+__device__ __forceinline__ void finish(const VerifyArgs &a, size_t b, uint32_t n, uint32_t len, uint64_t key) {
+    if (!key && n < len) {
+        const T *target = static_cast<const T *>(a.target) + b * a.target_batch + n * a.target_place;
+        key = block_largest<kRowThreads>(
+            race<T>(target, nullptr, a.noise + b * a.noise_batch, kNowhere, 0, a.vocab, kRowThreads));
     }
-    const uint64_t key = key_rest ? key_rest : key_all;
     const int64_t token = key ? (int64_t)(0xffffffffu - (uint32_t)key) : -1;
     for (uint32_t i = threadIdx.x; i <= a.K; i += kRowThreads) {
         const int64_t v = i < n ? whole(a.drafts, b * a.K + i, a.tokens64) : i == n ? token : -1;
@@ -357,7 +677,55 @@ k_verify(VerifyArgs a) {
         else
             static_cast<int32_t *>(a.tokens)[b * (a.K + 1) + i] = (int32_t)v;
     }
-    if (threadIdx.x == 0) a.accepted[b] = (int32_t)n;
+}
+
+// Draft i stays while u_i q_i(x_i) < p_i(x_i); the token after the first that does not is
+// drawn from max(p - q, 0), after the last one from p: the largest weight / noise, an
+// exponential race, has exactly that distribution, and needs no sum over the row, so the
+// stretches of a row are independent.  Each product, difference and quotient is one
+// rounding of 32 bits and a largest key has no order, so neither has the choice.
+template <class T>
+__global__ void __launch_bounds__(kRowThreads)
+k_verify(VerifyArgs a) {
+    const size_t job = row_of(), b = job / a.chunks;
+    if (b >= a.batch) return;
+    const uint32_t begin = (uint32_t)(job % a.chunks) * a.chunk, end = min(begin + a.chunk, a.vocab);
+    const uint32_t len = length_of(a, b), n = kept<T>(a, b, len);
+    const T *target = static_cast<const T *>(a.target) + b * a.target_batch + n * a.target_place;
+    const T *draft = a.draft && n < len
+                         ? static_cast<const T *>(a.draft) + b * a.draft_batch + n * a.draft_place
+                         : nullptr;
+    uint32_t without = kNowhere;
+    if (!a.draft && n < len) {
+        const int64_t x = whole(a.drafts, b * a.K + n, a.tokens64);
+        if (x >= 0 && x < (int64_t)a.vocab) without = (uint32_t)x;
+    }
+    const uint64_t key = block_largest<kRowThreads>(
+        race<T>(target, draft, a.noise + b * a.noise_batch, without, begin, end, kRowThreads));
+    if (a.chunks == 1) finish<T>(a, b, n, len, key);
+    if (threadIdx.x == 0) {
+        if (a.chunks > 1) a.parts[job] = key;
+        if (begin == 0) a.accepted[b] = (int32_t)n;
+    }
+}
+
+// joins the stretches of each sequence
+template <class T>
+__global__ void __launch_bounds__(kRowThreads)
+k_verify_join(VerifyArgs a) {
+    const size_t b = row_of();
+    if (b >= a.batch) return;
+    uint64_t key = 0;
+    for (uint32_t i = threadIdx.x; i < a.chunks; i += kRowThreads) key = larger(key, a.parts[b * a.chunks + i]);
+    key = block_largest<kRowThreads>(key);
+    finish<T>(a, b, (uint32_t)a.accepted[b], length_of(a, b), key);
+}
+
+Cut cut_race(size_t batch, uint32_t vocab) {
+    uint32_t chunk = 8 * kRowThreads * kVec;
+    if (vocab <= kRowThreads * kVec || batch >= 4096) return {vocab, 1};
+    while (chunk > kRowThreads * kVec && batch * ((vocab + chunk - 1) / chunk) < 1024) chunk /= 2;
+    return {chunk, (vocab + chunk - 1) / chunk};
 }
 
 constexpr size_t kMostWidth = (size_t)1 << 30;
@@ -448,13 +816,23 @@ int pfa_token_probabilities(const void *logits, size_t stride, int type, size_t 
         aligned(logits, size, "logits");
         aligned(out, 4, "out");
         aligned(temperatures, 4, "temperatures");
-        with_type(type, [&](auto t) {
-            using T = decltype(t);
-            hipLaunchKernelGGL(k_probabilities<T>, row_grid(rows), dim3(kRowThreads), 0, as_stream(stream),
-                               rows, (const T *)logits, stride, temperatures, (float)temperature, mask, mask_stride,
-                               (uint32_t)vocab, out);
-        });
+        const Cut cut = cut_probabilities(rows, (uint32_t)vocab);
+        const size_t need = cut.chunks == 1 ? 0 : rows * cut.chunks * sizeof(ProbPart);
+        require(workspace_bytes >= need, "pfa_token_probabilities: the workspace needs " + std::to_string(need) + " bytes");
+        aligned(workspace, 16, "workspace");
+        const ProbArgs a{logits, temperatures, mask, out, workspace, rows, stride, mask_stride, (uint32_t)vocab,
+                         cut.chunk, cut.chunks, (float)temperature};
+        with_type(type, [&](auto t) { probabilities<decltype(t)>(a, as_stream(stream)); });
         PFA_HIP(hipGetLastError());
+    });
+}
+
+int pfa_token_workspace(size_t rows, size_t vocab, size_t *bytes) {
+    return guarded([&] {
+        check_rows(rows, vocab, "pfa_token_workspace");
+        require(bytes != nullptr, "null argument");
+        const Cut p = cut_probabilities(rows, (uint32_t)vocab), v = cut_race(rows, (uint32_t)vocab);
+        *bytes = std::max(p.chunks == 1 ? 0 : rows * p.chunks * sizeof(ProbPart), v.chunks == 1 ? 0 : rows * v.chunks * 8);
     });
 }
 
@@ -481,12 +859,18 @@ int pfa_verify_drafts(const void *drafts, int token_bytes, const void *lengths, 
         aligned(uniforms, 4, "uniforms");
         aligned(noise, 4, "noise");
         aligned(accepted, 4, "accepted");
-        VerifyArgs a{drafts, lengths, target, draft, uniforms, noise, tokens, accepted, target_batch, target_place,
-                     draft_batch, draft_place, noise_batch, batch, (uint32_t)K, (uint32_t)vocab, token_bytes == 8,
-                     length_bytes == 8};
+        const Cut cut = cut_race(batch, (uint32_t)vocab);
+        const size_t need = cut.chunks == 1 ? 0 : batch * cut.chunks * 8;
+        require(workspace_bytes >= need, "pfa_verify_drafts: the workspace needs " + std::to_string(need) + " bytes");
+        aligned(workspace, 8, "workspace");
+        VerifyArgs a{drafts, lengths, target, draft, uniforms, noise, tokens, accepted, (uint64_t *)workspace,
+                     target_batch, target_place, draft_batch, draft_place, noise_batch, batch, (uint32_t)K,
+                     (uint32_t)vocab, cut.chunk, cut.chunks, token_bytes == 8, length_bytes == 8};
+        const hipStream_t s = as_stream(stream);
         with_type(type, [&](auto t) {
             using T = decltype(t);
-            hipLaunchKernelGGL(k_verify<T>, row_grid(batch), dim3(kRowThreads), 0, as_stream(stream), a);
+            hipLaunchKernelGGL(k_verify<T>, row_grid(batch * cut.chunks), dim3(kRowThreads), 0, s, a);
+            if (cut.chunks > 1) hipLaunchKernelGGL(k_verify_join<T>, row_grid(batch), dim3(kRowThreads), 0, s, a);
         });
         PFA_HIP(hipGetLastError());
     });

@@ -10,6 +10,7 @@ stream on the tensor's device.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -78,6 +79,7 @@ SIGNATURES = {
     "pfa_quantize_int8": (_i32, [_vp, _sz, _i32, _sz, _sz, _vp, _sz, _vp, _vp]),
     "pfa_rms_norm_int8": (_i32, [_vp, _sz, _vp, _sz, _vp, _i32, _sz, _sz, C.c_double, _vp, _sz, _vp, _sz, _vp, _vp]),
     "pfa_int8_matmul": (_i32, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _i32, _sz, _vp, _sz, _vp]),
+    "pfa_token_workspace": (_i32, [_sz, _sz, C.POINTER(_sz)]),
     "pfa_token_probabilities": (_i32, [_vp, _sz, _i32, _sz, _sz, _vp, C.c_double, _vp, _sz, _vp, _vp, _sz, _vp]),
     "pfa_verify_drafts": (_i32, [_vp, _i32, _vp, _i32, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _sz, _i32, _vp, _vp,
                                  _sz, _vp, _vp, _vp, _sz, _vp]),
@@ -180,6 +182,14 @@ def create_coeff_modulus(poly_degree: int, bit_sizes) -> list[int]:
     out = (C.c_uint64 * len(bit_sizes))()
     call("pfa_create_coeff_modulus", poly_degree, bits, len(bit_sizes), out)
     return [int(x) for x in out]
+
+
+@functools.lru_cache(maxsize=1024)
+def token_workspace(rows: int, vocab: int) -> int:
+    """Bytes of workspace for probabilities of, or a choice from, rows x vocab."""
+    n = C.c_size_t(0)
+    call("pfa_token_workspace", rows, vocab, C.byref(n))
+    return int(n.value)
 
 
 def galois_elt_from_step(step: int, poly_degree: int) -> int:
