@@ -338,9 +338,11 @@ __device__ __forceinline__ void write_nan(const uint8_t *mask, float *out, uint3
     for (uint32_t i = begin + threadIdx.x; i < end; i += threads) out[i] = !mask || mask[i] ? not_a_number() : 0.f;
 }
 
-// Rows in one piece: read once, reduced twice, written once.
+// Rows in one piece: read once, reduced twice, written once.  Two workgroups of 1024
+// threads on a CU (64 registers a lane) let one read while the other writes: 4096 rows of
+// 32768 bf16 in 167 us (4.8 TB/s), with one of them 203 us.
 template <class T, int THREADS, int STEPS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 && STEPS <= 4 ? 8 : 1)
 k_prob_rows(ProbArgs a) {
     const size_t row = row_of();
     if (row >= a.rows) return;
@@ -506,15 +508,16 @@ k_prob_short(ProbArgs a) {
 struct Cut {
     uint32_t chunk, chunks;
 };
+
+// One piece while a row's values fit the registers of 1024 threads, unless there are too
+// few rows for the card (measured, bf16, us, one piece / cut: 16 rows of 32768 8.0 / 6.9, 128
+// rows 11.7 / 13.4; 128 rows of 65536 20.2 / 18.9, 512 rows 50 / 57).  Stretches have one vector
+// a thread while that gives the card little to do, then two, which share a workgroup's
+// start and reductions (16 rows of 131072 10.0 / 9.9, 512 rows 127 / 114; four: 115).
 Cut cut_probabilities(size_t rows, uint32_t vocab) {
-    if (vocab < kVec) return {vocab, 1};
-    // one piece: up to 64 values a thread stay in registers.  Few long rows leave most of
-    // the card idle so, and are cut.
-    if (vocab <= 65536 && (rows >= 128 || vocab <= 8192)) return {vocab, 1};
-    uint32_t steps = 8;
-    while (steps > 1 && rows * ((vocab + steps * kChunkThreads * kVec - 1) / (steps * kChunkThreads * kVec)) < 1024)
-        steps /= 2;
-    const uint32_t chunk = steps * kChunkThreads * kVec;
+    if (vocab <= 16384 || (vocab <= 32768 && rows >= 64) || (vocab <= 65536 && rows >= 256)) return {vocab, 1};
+    const uint32_t least = kChunkThreads * kVec;
+    const uint32_t chunk = rows * ((vocab + least - 1) / least) < 1024 ? least : 2 * least;
     return {chunk, (vocab + chunk - 1) / chunk};
 }
 
@@ -534,29 +537,19 @@ void probabilities(const ProbArgs &a, hipStream_t s) {
         else if (vecs <= 1024)
             PFA_LAUNCH((k_prob_rows<T, 256, 4>), a.rows, 256);
         else if (vecs <= 2048)
-            PFA_LAUNCH((k_prob_rows<T, 256, 8>), a.rows, 256);
+            PFA_LAUNCH((k_prob_rows<T, 1024, 2>), a.rows, 1024);
         else if (vecs <= 4096)
             PFA_LAUNCH((k_prob_rows<T, 1024, 4>), a.rows, 1024);
         else
             PFA_LAUNCH((k_prob_rows<T, 1024, 8>), a.rows, 1024);
     } else {
         const size_t jobs = a.rows * a.chunks;
-        switch (a.chunk / (kChunkThreads * kVec)) {
-            case 1:
-                PFA_LAUNCH((k_prob_parts<T, 1>), jobs, kChunkThreads);
-                PFA_LAUNCH((k_prob_write<T, 1>), jobs, kChunkThreads);
-                break;
-            case 2:
-                PFA_LAUNCH((k_prob_parts<T, 2>), jobs, kChunkThreads);
-                PFA_LAUNCH((k_prob_write<T, 2>), jobs, kChunkThreads);
-                break;
-            case 4:
-                PFA_LAUNCH((k_prob_parts<T, 4>), jobs, kChunkThreads);
-                PFA_LAUNCH((k_prob_write<T, 4>), jobs, kChunkThreads);
-                break;
-            default:
-                PFA_LAUNCH((k_prob_parts<T, 8>), jobs, kChunkThreads);
-                PFA_LAUNCH((k_prob_write<T, 8>), jobs, kChunkThreads);
+        if (a.chunk == kChunkThreads * kVec) {
+            PFA_LAUNCH((k_prob_parts<T, 1>), jobs, kChunkThreads);
+            PFA_LAUNCH((k_prob_write<T, 1>), jobs, kChunkThreads);
+        } else {
+            PFA_LAUNCH((k_prob_parts<T, 2>), jobs, kChunkThreads);
+            PFA_LAUNCH((k_prob_write<T, 2>), jobs, kChunkThreads);
         }
     }
 #undef PFA_LAUNCH
@@ -721,10 +714,12 @@ k_verify_join(VerifyArgs a) {
     finish<T>(a, b, (uint32_t)a.accepted[b], length_of(a, b), key);
 }
 
-Cut cut_race(size_t batch, uint32_t vocab) {
-    uint32_t chunk = 8 * kRowThreads * kVec;
-    if (vocab <= kRowThreads * kVec || batch >= 4096) return {vocab, 1};
-    while (chunk > kRowThreads * kVec && batch * ((vocab + chunk - 1) / chunk) < 1024) chunk /= 2;
+// Stretches of one vector a thread (64 sequences of 100003: 19.0 us, of eight 19.6; one of
+// 131072: 5.8 and 10.2), unless a row is so short that a workgroup takes it as fast
+// (8192 places, 1 sequence: 5.8 us either way; 256: 8.3 in one piece, 10.5 cut).
+Cut cut_race(uint32_t vocab) {
+    const uint32_t chunk = kRowThreads * kVec;
+    if (vocab <= 4 * chunk) return {vocab, 1};
     return {chunk, (vocab + chunk - 1) / chunk};
 }
 
@@ -831,7 +826,7 @@ int pfa_token_workspace(size_t rows, size_t vocab, size_t *bytes) {
     return guarded([&] {
         check_rows(rows, vocab, "pfa_token_workspace");
         require(bytes != nullptr, "null argument");
-        const Cut p = cut_probabilities(rows, (uint32_t)vocab), v = cut_race(rows, (uint32_t)vocab);
+        const Cut p = cut_probabilities(rows, (uint32_t)vocab), v = cut_race((uint32_t)vocab);
         *bytes = std::max(p.chunks == 1 ? 0 : rows * p.chunks * sizeof(ProbPart), v.chunks == 1 ? 0 : rows * v.chunks * 8);
     });
 }
@@ -859,7 +854,7 @@ int pfa_verify_drafts(const void *drafts, int token_bytes, const void *lengths, 
         aligned(uniforms, 4, "uniforms");
         aligned(noise, 4, "noise");
         aligned(accepted, 4, "accepted");
-        const Cut cut = cut_race(batch, (uint32_t)vocab);
+        const Cut cut = cut_race((uint32_t)vocab);
         const size_t need = cut.chunks == 1 ? 0 : batch * cut.chunks * 8;
         require(workspace_bytes >= need, "pfa_verify_drafts: the workspace needs " + std::to_string(need) + " bytes");
         aligned(workspace, 8, "workspace");
