@@ -422,11 +422,14 @@ int pfa_rms_norm_int8(const void *x, size_t x_stride, const void *residual, size
                       const void *weight, int type, size_t rows, size_t width, double eps, void *total,
                       size_t total_stride, int8_t *codes, size_t codes_stride, float *scales, void *stream);
 
+/* Bytes of workspace that pfa_int8_matmul needs for these sizes (0: none). */
+int pfa_matmul_workspace(size_t M, size_t N, size_t K, size_t *bytes);
+
 /* out[m][n] = (sum_k a[m][k] b[n][k]) a_scales[m] b_scales[n] + bias[n] (bias NULL:
  * none), out of `type`.  a [M][K], b [N][K].  The sums are exact: K <= 131071.
  * Rows of a and b that start at multiples of 16 bytes are read fastest.
- * workspace: `workspace_bytes` of device memory, 16-byte aligned, that no other
- * call in flight uses, or NULL and 0. */
+ * workspace: pfa_matmul_workspace bytes of device memory, 16-byte aligned, that no
+ * other call in flight uses (NULL where that is 0). */
 int pfa_int8_matmul(const int8_t *a, size_t a_stride, const float *a_scales, const int8_t *b, size_t b_stride,
                     const float *b_scales, const float *bias, size_t M, size_t N, size_t K, void *out, int type,
                     size_t out_stride, void *workspace, size_t workspace_bytes, void *stream);

@@ -21,6 +21,9 @@ import pfa_native as _N
 __all__ = ["quantize_int8", "rms_norm_int8", "int8_matmul", "token_probabilities", "verify_drafts"]
 
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PFA_F32, PFA_BF16, PFA_F16
+# the handle of the current stream of a device: torch.cuda.current_stream without the object
+# around it, which costs a call of a few microseconds more than its launch
+_raw_stream = torch._C._cuda_getCurrentRawStream
 _WHOLE = {torch.int32: 4, torch.int64: 8}
 
 
@@ -36,21 +39,25 @@ def _type_of(t, name):
 
 
 def _same_device(first, **others):
+    index = first.get_device()
     if not first.is_cuda:
         _fail("expected tensors on a GPU")
     for name, t in others.items():
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
             _fail(f"{name} is on {t.device}, not on {first.device}")
 
 
 def _call(name, t, *args):
     """The entry point on t's device and its current stream."""
-    device = t.device.index
-    if device == torch.cuda.current_device():
-        _N.call(name, *args, _N.stream_of(t))
+    index = t.get_device()
+    f = getattr(_N.lib(), name)
+    if index == torch.cuda.current_device():
+        rc = f(*args, _raw_stream(index) or _N.HIP_STREAM_LEGACY)
     else:
-        with torch.cuda.device(device):
-            _N.call(name, *args, _N.stream_of(t))
+        with torch.cuda.device(index):
+            rc = f(*args, _raw_stream(index) or _N.HIP_STREAM_LEGACY)
+    if rc:
+        _N.check(rc)
 
 
 def _matrix(t, name):
@@ -80,9 +87,8 @@ def _new_codes(shape, device):
     return torch.empty((*shape[:-1], -(-width // 16) * 16), dtype=torch.int8, device=device)[..., :width]
 
 
-def _workspace(rows, vocab, device):
-    """(tensor to hold on to, address, bytes) of the workspace of a row of places for each of rows."""
-    need = _N.token_workspace(rows, vocab)
+def _workspace(need, device):
+    """(tensor to hold on to, address, bytes) of a call's workspace."""
     if not need:
         return None, None, 0
     t = torch.empty((need,), dtype=torch.uint8, device=device)
@@ -170,9 +176,10 @@ def int8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
         _vector(bias, n, torch.float32, "bias")
     out = torch.empty((*a.shape[:-1], n), dtype=out_dtype, device=a.device)
     if m and n:
+        held, space, size = _workspace(_N.matmul_workspace(m, n, k), out.device)
         _call("pfa_int8_matmul", a, rows.data_ptr(), a_stride, a_scales.data_ptr(), cols.data_ptr(), b_stride,
               b_scales.data_ptr(), bias.data_ptr() if bias is not None else None, m, n, k, out.data_ptr(), kind, n,
-              None, 0)
+              space, size)
     return out
 
 
@@ -212,7 +219,7 @@ def token_probabilities(logits, temperature=1.0, mask=None):
     _same_device(logits, temperature=temperatures, mask=mask)
     out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
     if out.numel():
-        held, space, size = _workspace(n, vocab, out.device)
+        held, space, size = _workspace(_N.token_workspace(n, vocab), out.device)
         _call("pfa_token_probabilities", logits, rows.data_ptr(), stride, kind, n, vocab,
               temperatures.data_ptr() if temperatures is not None else None, one,
               allowed.data_ptr() if allowed is not None else None, mask_stride, out.data_ptr(), space, size)
@@ -278,7 +285,7 @@ def verify_drafts(draft_tokens, target_probs, uniforms, noise, draft_probs=None,
     tokens = torch.empty((batch, places), dtype=draft_tokens.dtype, device=target_probs.device)
     accepted = torch.empty((batch,), dtype=torch.int32, device=target_probs.device)
     if batch:
-        held, space, need = _workspace(batch, vocab, tokens.device)
+        held, space, need = _workspace(_N.token_workspace(batch, vocab), tokens.device)
         _call("pfa_verify_drafts", target_probs, draft_tokens.data_ptr(), size,
               lengths.data_ptr() if lengths is not None else None, length_size, batch, drafts, vocab,
               target_probs.data_ptr(), target_batch, target_place,

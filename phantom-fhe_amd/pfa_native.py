@@ -78,6 +78,7 @@ SIGNATURES = {
     "pfa_ct_lincomb": (_i32, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _vp, _vp, _vp]),
     "pfa_quantize_int8": (_i32, [_vp, _sz, _i32, _sz, _sz, _vp, _sz, _vp, _vp]),
     "pfa_rms_norm_int8": (_i32, [_vp, _sz, _vp, _sz, _vp, _i32, _sz, _sz, C.c_double, _vp, _sz, _vp, _sz, _vp, _vp]),
+    "pfa_matmul_workspace": (_i32, [_sz, _sz, _sz, C.POINTER(_sz)]),
     "pfa_int8_matmul": (_i32, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _i32, _sz, _vp, _sz, _vp]),
     "pfa_token_workspace": (_i32, [_sz, _sz, C.POINTER(_sz)]),
     "pfa_token_probabilities": (_i32, [_vp, _sz, _i32, _sz, _sz, _vp, C.c_double, _vp, _sz, _vp, _vp, _sz, _vp]),
@@ -190,6 +191,14 @@ def token_workspace(rows: int, vocab: int) -> int:
     n = C.c_size_t(0)
     call("pfa_token_workspace", rows, vocab, C.byref(n))
     return int(n.value)
+
+
+@functools.lru_cache(maxsize=1024)
+def matmul_workspace(m: int, n: int, k: int) -> int:
+    """Bytes of workspace of int8_matmul for these sizes."""
+    size = C.c_size_t(0)
+    call("pfa_matmul_workspace", m, n, k, C.byref(size))
+    return int(size.value)
 
 
 def galois_elt_from_step(step: int, poly_degree: int) -> int:
