@@ -61,16 +61,19 @@ def _call(name, t, *args):
 
 
 def _matrix(t, name):
-    """t as (two-dimensional view of its rows, distance between them)."""
-    if t.dim() < 1:
-        _fail(f"{name} needs at least one dimension")
+    """(t as a two-dimensional view of its rows, distance between them)."""
     if t.dim() != 2:
+        if t.dim() < 1:
+            _fail(f"{name} needs at least one dimension")
         t = t.reshape(-1, t.shape[-1]) if t.numel() else t.new_empty((t.shape[:-1].numel(), t.shape[-1]))
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    (rows, width), (stride, inner) = t.shape, t.stride()
+    if inner != 1 and width > 1:
         _fail(f"{name}: the elements of a row must be adjacent")
-    if t.shape[0] > 1 and 0 < t.stride(0) < t.shape[1]:
+    if rows <= 1:
+        return t, width
+    if 0 < stride < width:
         _fail(f"{name}: rows overlap")
-    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return t, stride
 
 
 def _vector(t, n, dtype, name):
@@ -79,19 +82,31 @@ def _vector(t, n, dtype, name):
     return t
 
 
-def _new_codes(shape, device):
-    """Codes whose rows start at multiples of 16 bytes, which int8_matmul reads fastest."""
+def _new(like, shape, dtype):
+    """An empty contiguous tensor on like's device (the strided call is the cheapest of torch's)."""
+    strides, n = [], 1
+    for size in reversed(shape):
+        strides.append(n)
+        n *= size or 1
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=like.device)
+
+
+def _new_codes(like):
+    """(codes of like's shape, distance of their rows): rows start at multiples of 16 bytes,
+    which int8_matmul reads fastest."""
+    shape = like.shape
     width = shape[-1]
-    if width % 16 == 0:
-        return torch.empty(shape, dtype=torch.int8, device=device)
-    return torch.empty((*shape[:-1], -(-width // 16) * 16), dtype=torch.int8, device=device)[..., :width]
+    stride = (width + 15) & ~15
+    if stride == width:
+        return _new(like, shape, torch.int8), width
+    return _new(like, (*shape[:-1], stride), torch.int8)[..., :width], stride
 
 
 def _workspace(need, device):
     """(tensor to hold on to, address, bytes) of a call's workspace."""
     if not need:
         return None, None, 0
-    t = torch.empty((need,), dtype=torch.uint8, device=device)
+    t = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device)
     return t, t.data_ptr(), need
 
 
@@ -107,11 +122,12 @@ def quantize_int8(x):
     kind = _type_of(x, "x")
     _same_device(x)
     rows, stride = _matrix(x, "x")
-    codes = _new_codes(x.shape, x.device)
-    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    if scales.numel():
-        _call("pfa_quantize_int8", x, rows.data_ptr(), stride, kind, rows.shape[0], rows.shape[1], codes.data_ptr(),
-              _matrix(codes, "codes")[1], scales.data_ptr())
+    codes, codes_stride = _new_codes(x)
+    scales = _new(x, x.shape[:-1], torch.float32)
+    n, width = rows.shape
+    if n:
+        _call("pfa_quantize_int8", x, rows.data_ptr(), stride, kind, n, width, codes.data_ptr(), codes_stride,
+              scales.data_ptr())
     return codes, scales
 
 
@@ -137,13 +153,13 @@ def rms_norm_int8(x, weight, eps=1e-6, residual=None):
         if residual.shape != x.shape or residual.dtype != x.dtype:
             _fail(f"residual: expected {tuple(x.shape)} of {x.dtype}, got {tuple(residual.shape)} of {residual.dtype}")
         more, more_stride = _matrix(residual, "residual")
-        total, total_stride = torch.empty(x.shape, dtype=x.dtype, device=x.device), width
-    codes = _new_codes(x.shape, x.device)
-    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        total, total_stride = _new(x, x.shape, x.dtype), width
+    codes, codes_stride = _new_codes(x)
+    scales = _new(x, x.shape[:-1], torch.float32)
     if n:
         _call("pfa_rms_norm_int8", x, rows.data_ptr(), stride, more.data_ptr() if more is not None else None,
               more_stride, weight.data_ptr(), kind, n, width, float(eps), total.data_ptr() if total_stride else None,
-              total_stride, codes.data_ptr(), _matrix(codes, "codes")[1], scales.data_ptr())
+              total_stride, codes.data_ptr(), codes_stride, scales.data_ptr())
     return codes, scales, total
 
 
@@ -174,7 +190,7 @@ def int8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
     _vector(b_scales, n, torch.float32, "b_scales")
     if bias is not None:
         _vector(bias, n, torch.float32, "bias")
-    out = torch.empty((*a.shape[:-1], n), dtype=out_dtype, device=a.device)
+    out = _new(a, (*a.shape[:-1], n), out_dtype)
     if m and n:
         held, space, size = _workspace(_N.matmul_workspace(m, n, k), out.device)
         _call("pfa_int8_matmul", a, rows.data_ptr(), a_stride, a_scales.data_ptr(), cols.data_ptr(), b_stride,
@@ -217,7 +233,7 @@ def token_probabilities(logits, temperature=1.0, mask=None):
         else:
             allowed = mask
     _same_device(logits, temperature=temperatures, mask=mask)
-    out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+    out = _new(logits, logits.shape, torch.float32)
     if out.numel():
         held, space, size = _workspace(_N.token_workspace(n, vocab), out.device)
         _call("pfa_token_probabilities", logits, rows.data_ptr(), stride, kind, n, vocab,
@@ -282,8 +298,8 @@ def verify_drafts(draft_tokens, target_probs, uniforms, noise, draft_probs=None,
         if length_size is None or lengths.shape != (batch,) or not lengths.is_contiguous():
             _fail(f"lengths: expected {batch} adjacent values of int32 or int64, got {tuple(lengths.shape)} of "
                   f"{lengths.dtype}")
-    tokens = torch.empty((batch, places), dtype=draft_tokens.dtype, device=target_probs.device)
-    accepted = torch.empty((batch,), dtype=torch.int32, device=target_probs.device)
+    tokens = _new(target_probs, (batch, places), draft_tokens.dtype)
+    accepted = _new(target_probs, (batch,), torch.int32)
     if batch:
         held, space, need = _workspace(_N.token_workspace(batch, vocab), tokens.device)
         _call("pfa_verify_drafts", target_probs, draft_tokens.data_ptr(), size,

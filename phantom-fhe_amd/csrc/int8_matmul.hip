@@ -50,90 +50,60 @@ __device__ __forceinline__ i32x4 load16_end(const int8_t *row, uint32_t k, uint3
     return v;
 }
 
-// Few rows of a: b is streamed once, so its bytes are the time.  A workgroup takes
-// NT x 16 columns and all rows (MT x 16 of them), its waves take blocks of 128 codes of K
-// in turn and meet in LDS, where integer additions have no order.  In a block a lane
-// takes 32 neighbouring codes of one row: two matrix instructions, which may see K in
-// any order as long as both operands agree, and every line of b is read whole.
+// Up to 16 rows of a: b is streamed once, so its bytes are the time.  A workgroup takes
+// 16 columns and all rows, its waves take blocks of 128 codes of K in turn and meet in LDS,
+// where integer additions have no order.  In a block a lane takes 32 neighbouring codes
+// of one row: two matrix instructions, which may see K in any order as long as both
+// operands agree, and every line of b is read whole.  One row, 16384 columns, K = 4096:
+// 15.3 us (4.4 TB/s); 4096 columns: 6.2 us.  More rows or columns a wave were slower: a's
+// fragments come through the vector cache, whose time then exceeds b's.
 constexpr int kBlock = 128;
+constexpr int kFewWaves = 8, kFewUnroll = 4;  // four blocks a wave in flight
 
-template <class T, int MT, int NT, int WAVES, int UNROLL>
-__global__ void __launch_bounds__(WAVES * 64)
+template <class T>
+__global__ void __launch_bounds__(kFewWaves * 64)
 k_few_rows(MatmulArgs g) {
-    __shared__ int sums[MT * 16][NT * 16];
+    __shared__ int sums[16][16];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const uint32_t n0 = blockIdx.x * (NT * 16);
-    for (uint32_t i = threadIdx.x; i < MT * 16 * NT * 16; i += WAVES * 64) sums[0][i] = 0;
-    const int8_t *pa[MT], *pb[NT];
+    const uint32_t n0 = blockIdx.x * 16;
+    if (threadIdx.x < 256) sums[0][threadIdx.x] = 0;
     const uint32_t at = lane / 16 * 32;
-#pragma unroll
-    for (int m = 0; m < MT; m++) pa[m] = g.a + (size_t)min(m * 16 + lane % 16, g.M - 1) * g.a_stride;
-#pragma unroll
-    for (int n = 0; n < NT; n++) pb[n] = g.b + (size_t)min(n0 + n * 16 + lane % 16, g.N - 1) * g.b_stride;
-    i32x4 acc[MT][NT];
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int n = 0; n < NT; n++) acc[m][n] = {0, 0, 0, 0};
+    const int8_t *pa = g.a + (size_t)min(lane % 16, g.M - 1) * g.a_stride;
+    const int8_t *pb = g.b + (size_t)min(n0 + lane % 16, g.N - 1) * g.b_stride;
+    i32x4 acc = {0, 0, 0, 0};
     const uint32_t blocks = g.K / kBlock;
     uint32_t k = wave;
-    for (; k + (UNROLL - 1) * WAVES < blocks; k += UNROLL * WAVES) {
-        i32x4 fa[UNROLL][MT][2], fb[UNROLL][NT][2];
+    for (; k + (kFewUnroll - 1) * kFewWaves < blocks; k += kFewUnroll * kFewWaves) {
+        i32x4 fa[kFewUnroll][2], fb[kFewUnroll][2];
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
-            const uint32_t c = (k + u * WAVES) * kBlock + at;
+        for (int u = 0; u < kFewUnroll; u++)
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                fb[u][n][0] = load16(pb[n], c);
-                fb[u][n][1] = load16(pb[n], c + 16);
+            for (int h = 0; h < 2; h++) {
+                const uint32_t c = (k + u * kFewWaves) * kBlock + at + h * 16;
+                fb[u][h] = load16(pb, c);
+                fa[u][h] = load16(pa, c);
             }
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-                fa[u][m][0] = load16(pa[m], c);
-                fa[u][m][1] = load16(pa[m], c + 16);
-            }
-        }
+        for (int u = 0; u < kFewUnroll; u++)
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++)
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        acc[m][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[u][n][h], fa[u][m][h], acc[m][n], 0, 0, 0);
+            for (int h = 0; h < 2; h++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[u][h], fa[u][h], acc, 0, 0, 0);
     }
-    // what is left: whole blocks, and the wave whose turn it is takes the row's end
-    for (; k * kBlock < g.K; k += WAVES) {
+    // what is left: whole blocks, and the wave whose turn it is takes the rows' end
+    for (; k * kBlock < g.K; k += kFewWaves) {
         const uint32_t c = k * kBlock + at;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            i32x4 fa[MT], fb[NT];
-#pragma unroll
-            for (int n = 0; n < NT; n++) fb[n] = load16_end(pb[n], c + h * 16, g.K);
-#pragma unroll
-            for (int m = 0; m < MT; m++) fa[m] = load16_end(pa[m], c + h * 16, g.K);
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-                    acc[m][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[n], fa[m], acc[m][n], 0, 0, 0);
-        }
+        for (int h = 0; h < 2; h++)
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(load16_end(pb, c + h * 16, g.K), load16_end(pa, c + h * 16, g.K),
+                                                        acc, 0, 0, 0);
     }
     __syncthreads();
 #pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) atomicAdd(&sums[m * 16 + lane % 16][n * 16 + lane / 16 * 4 + i], acc[m][n][i]);
+    for (int i = 0; i < 4; i++) atomicAdd(&sums[lane % 16][lane / 16 * 4 + i], acc[i]);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < MT * 16 * NT * 16; i += WAVES * 64) {
-        const uint32_t m = i / (NT * 16), n = n0 + i % (NT * 16);
-        if (m < g.M && n < g.N)
-            static_cast<T *>(g.out)[(size_t)m * g.out_stride + n] =
-                (T)((float)sums[0][i] * g.sa[m] * g.sb[n] + (g.bias ? g.bias[n] : 0.f));
-    }
+    const uint32_t m = threadIdx.x / 16, n = n0 + threadIdx.x % 16;
+    if (m < g.M && threadIdx.x < 256 && n < g.N)
+        static_cast<T *>(g.out)[(size_t)m * g.out_stride + n] =
+            (T)((float)sums[m][threadIdx.x % 16] * g.sa[m] * g.sb[n] + (g.bias ? g.bias[n] : 0.f));
 }
 
 // Many rows: BM x BN outputs a workgroup of WM x WN waves.  Blocks of 128 codes of K go
@@ -440,7 +410,7 @@ void launch_tiles(const MatmulArgs &g, hipStream_t s) {
 template <class T>
 void matmul(const MatmulArgs &g, const Plan &p, hipStream_t s) {
     if (p.few) {
-        hipLaunchKernelGGL((k_few_rows<T, 1, 1, 8, 4>), dim3((g.N + 15) / 16), dim3(512), 0, s, g);
+        hipLaunchKernelGGL(k_few_rows<T>, dim3((g.N + 15) / 16), dim3(kFewWaves * 64), 0, s, g);
         return;
     }
     switch (p.shape) {

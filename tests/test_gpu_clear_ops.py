@@ -583,3 +583,19 @@ def test_same_call_same_bits(dev):
         want = step(*ins)
         for _ in range(5):
             assert all(torch.equal(a, b) for a, b in zip(step(*ins), want))
+
+
+def test_example(dev):
+    """examples/encrypted_decoding.py: an encrypted layer between drafts and their check."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "encrypted_decoding.py")
+    spec = importlib.util.spec_from_file_location("encrypted_decoding", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    text, worst = module.run(rounds=2, say=lambda _: None)
+    assert 2 <= len(text) <= 10 and all(0 <= t < 1000 for t in text)
+    # codes are off by half a step of 1/127 of their row's largest, about 4 deviations: logits of deviation 1 by
+    # 0.013 (normal) in each factor, so probabilities by 0.02 / 0.8, half of it in total variation
+    assert worst < 0.03
