@@ -24,6 +24,7 @@ _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PFA_F32, PFA_
 # the handle of the current stream of a device: torch.cuda.current_stream without the object
 # around it, which costs a call of a few microseconds more than its launch
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
 _WHOLE = {torch.int32: 4, torch.int64: 8}
 
 
@@ -38,20 +39,25 @@ def _type_of(t, name):
     return code
 
 
-def _same_device(first, **others):
-    index = first.get_device()
+def _same_device(first, *others):
     if not first.is_cuda:
         _fail("expected tensors on a GPU")
-    for name, t in others.items():
+    index = first.get_device()
+    for t in others:
         if t is not None and t.get_device() != index:
-            _fail(f"{name} is on {t.device}, not on {first.device}")
+            _fail(f"tensors on {first.device} and on {t.device}")
+
+
+_entries = {}
 
 
 def _call(name, t, *args):
     """The entry point on t's device and its current stream."""
+    f = _entries.get(name)
+    if f is None:
+        f = _entries[name] = getattr(_N.lib(), name)
     index = t.get_device()
-    f = getattr(_N.lib(), name)
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         rc = f(*args, _raw_stream(index) or _N.HIP_STREAM_LEGACY)
     else:
         with torch.cuda.device(index):
@@ -84,11 +90,14 @@ def _vector(t, n, dtype, name):
 
 def _new(like, shape, dtype):
     """An empty contiguous tensor on like's device (the strided call is the cheapest of torch's)."""
-    strides, n = [], 1
-    for size in reversed(shape):
-        strides.append(n)
-        n *= size or 1
-    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=like.device)
+    dims = len(shape)
+    if dims == 2 and shape[1]:
+        strides = (shape[1], 1)
+    elif dims == 1:
+        strides = (1,)
+    else:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    return torch.empty_strided(shape, strides, dtype=dtype, device=like.device)
 
 
 def _new_codes(like):
@@ -140,7 +149,7 @@ def rms_norm_int8(x, weight, eps=1e-6, residual=None):
     the unrounded y.  x [..., width]; residual like x; weight [width]; all of one type.
     """
     kind = _type_of(x, "x")
-    _same_device(x, weight=weight, residual=residual)
+    _same_device(x, weight, residual)
     if not eps >= 0:
         _fail("eps must be 0 or more")
     rows, stride = _matrix(x, "x")
@@ -177,7 +186,7 @@ def int8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
         _fail(f"out_dtype: expected float32, bfloat16 or float16, got {out_dtype}")
     if a.dtype != torch.int8 or b.dtype != torch.int8:
         _fail(f"expected int8 codes, got {a.dtype} and {b.dtype}")
-    _same_device(a, a_scales=a_scales, b=b, b_scales=b_scales, bias=bias)
+    _same_device(a, a_scales, b, b_scales, bias)
     if b.dim() != 2 or a.dim() < 1 or a.shape[-1] != b.shape[1]:
         _fail(f"shapes {tuple(a.shape)} and {tuple(b.shape)} do not multiply")
     if a_scales.dtype != torch.float32 or a_scales.shape != a.shape[:-1] or not a_scales.is_contiguous():
@@ -232,7 +241,7 @@ def token_probabilities(logits, temperature=1.0, mask=None):
             allowed, mask_stride = _matrix(mask, "mask")
         else:
             allowed = mask
-    _same_device(logits, temperature=temperatures, mask=mask)
+    _same_device(logits, temperatures, mask)
     out = _new(logits, logits.shape, torch.float32)
     if out.numel():
         held, space, size = _workspace(_N.token_workspace(n, vocab), out.device)
@@ -265,8 +274,7 @@ def verify_drafts(draft_tokens, target_probs, uniforms, noise, draft_probs=None,
     size = _WHOLE.get(draft_tokens.dtype)
     if size is None:
         _fail(f"draft_tokens: expected int32 or int64, got {draft_tokens.dtype}")
-    _same_device(target_probs, draft_tokens=draft_tokens, uniforms=uniforms, noise=noise, draft_probs=draft_probs,
-                 lengths=lengths)
+    _same_device(target_probs, draft_tokens, uniforms, noise, draft_probs, lengths)
     if target_probs.dim() != 3 or target_probs.shape[1] < 1:
         _fail(f"target_probs: expected [batch, drafts + 1, vocab], got {tuple(target_probs.shape)}")
     batch, places, vocab = target_probs.shape

@@ -3,6 +3,8 @@
 //   out[m][n] = (sum_k a[m][k] b[n][k]) sa[m] sb[n] + bias[n]
 // Sums are exact in 32-bit integers for K <= 131071 (128^2 K < 2^31); the scales
 // are applied in 32-bit floats, and one rounding leads to the output's type.
+#include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <type_traits>
 
@@ -32,22 +34,28 @@ __device__ __forceinline__ i32x4 load16(const int8_t *row, uint32_t k) {
     return v;
 }
 __device__ __forceinline__ i32x4 load16_end(const int8_t *row, uint32_t k, uint32_t K) {
-    i32x4 v = {0, 0, 0, 0};
-    if (k + 16 <= K) {
-        v = load16(row, k);
-    } else if (k < K && K >= 16) {
-        // the row's last 16 codes, moved down to the bytes before k + 16
-        const i32x4 l = load16(row, K - 16);
-        const uint32_t s = k + 16 - K;
-        const u128 w = ((u128)(uint32_t)l[3] << 96 | (u128)(uint32_t)l[2] << 64 | (u128)(uint32_t)l[1] << 32 |
-                        (uint32_t)l[0]) >> (s * 8);
-        v = {(int)(uint32_t)w, (int)(uint32_t)(w >> 32), (int)(uint32_t)(w >> 64), (int)(uint32_t)(w >> 96)};
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (k + i < K) v[i / 4] |= (int)((uint32_t)(uint8_t)row[k + i] << (i % 4 * 8));
+    if (K < 16) {
+        i32x4 v = {0, 0, 0, 0};
+#pragma unroll 1
+        for (uint32_t i = k; i < K; i++) {
+            const int c = (int)((uint32_t)(uint8_t)row[i] << (i % 4 * 8));
+            v[0] |= i / 4 == k / 4 ? c : 0;
+            v[1] |= i / 4 == k / 4 + 1 ? c : 0;
+            v[2] |= i / 4 == k / 4 + 2 ? c : 0;
+            v[3] |= i / 4 == k / 4 + 3 ? c : 0;
+        }
+        return v;
     }
-    return v;
+    // past the end: the row's last 16 codes, moved down by what is past
+    const uint32_t at = min(k, K - 16), past = min(k - at, 16u);
+    i32x4 v = load16(row, at);
+    if (past & 8) v = {v[2], v[3], 0, 0};
+    if (past & 4) v = {v[1], v[2], v[3], 0};
+    const uint32_t bits = past % 4 * 8;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        v[i] = (int)__builtin_amdgcn_alignbit(i < 3 ? (uint32_t)v[i + 1] : 0u, (uint32_t)v[i], bits);
+    return past & 16 ? i32x4{0, 0, 0, 0} : v;
 }
 
 // Up to 16 rows of a: b is streamed once, so its bytes are the time.  A workgroup takes
@@ -362,25 +370,27 @@ struct Plan {
     uint32_t splits;
 };
 
-// The plan of least estimated time.  Few rows and few columns: k_few_rows (1 x 8192 x 2048: 6.3 us,
+// The plan of least estimated time: that of the products, or of reading b, a little more for every
+// row of tiles that reads it again.  Few rows and few columns go to k_few_rows (1 x 8192 x 2048: 6.3 us,
 // tiles 6.7; 1 x 32768 x 2048: 16 us, tiles 14).  K is split where tiles are too few for the card and the sums are
 // long enough to pay for the second launch and the partial sums (64 x 2048 x 8192: 15 us whole, 11 us in 4).
 Plan plan_matmul(size_t M, size_t N, size_t K) {
     if (M <= 16 && N <= 16384) return {true, 0, 1};
-    const float blocks = (float)((K + kBlock - 1) / kBlock);
+    const float blocks = (float)((K + kBlock - 1) / kBlock), memory = 5e6f;  // bytes a us
     Plan best{false, 0, 1};
-    float least = 0;
+    float least = INFINITY;
     for (int i = 0; i < kShapes; i++) {
         const Shape &s = shapes[i];
-        if (i && s.rows > 32 && M <= s.rows / 2) continue;  // half a tile or more of nothing
-        const size_t tiles = ((M + s.rows - 1) / s.rows) * ((N + s.cols - 1) / s.cols);
+        if (s.rows > 32 && M <= s.rows / 2) continue;  // half a tile or more of nothing
+        const size_t down = (M + s.rows - 1) / s.rows, tiles = down * ((N + s.cols - 1) / s.cols);
+        const float reading = ((float)N * K * (1 + .15f * (down - 1)) + (float)M * K) / memory;
         for (uint32_t splits = 1; splits <= 8; splits *= 2) {
             if (splits > 1 && (tiles * splits > 512 || blocks < 8 * splits)) break;
             const size_t on_cu = (tiles * splits + 255) / 256;
             const float block = on_cu <= 1 ? s.alone : on_cu == 2 ? s.pair : on_cu * s.each;
-            const float join = splits == 1 ? 0.f : 4.f + (float)splits * M * N * 8 / 4e6f;
-            const float time = block * blocks / splits + join;
-            if ((i == 0 && splits == 1) || time < least) {
+            const float join = splits == 1 ? 0.f : 4.f + (float)splits * M * N * 8 / memory;
+            const float time = std::max(block * blocks / splits, reading) + join;
+            if (time < least) {
                 least = time;
                 best = {false, i, splits};
             }
