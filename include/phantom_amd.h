@@ -427,7 +427,7 @@ int pfa_matmul_workspace(size_t M, size_t N, size_t K, size_t *bytes);
 
 /* out[m][n] = (sum_k a[m][k] b[n][k]) a_scales[m] b_scales[n] + bias[n] (bias NULL:
  * none), out of `type`.  a [M][K], b [N][K].  The sums are exact: K <= 131071.
- * Rows of a and b that start at multiples of 16 bytes are read fastest.
+ * Rows of a and b that start at multiples of 128 bytes are read fastest.
  * workspace: pfa_matmul_workspace bytes of device memory, 16-byte aligned, that no
  * other call in flight uses (NULL where that is 0). */
 int pfa_int8_matmul(const int8_t *a, size_t a_stride, const float *a_scales, const int8_t *b, size_t b_stride,

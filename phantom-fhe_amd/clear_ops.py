@@ -101,11 +101,11 @@ def _new(like, shape, dtype):
 
 
 def _new_codes(like):
-    """(codes of like's shape, distance of their rows): rows start at multiples of 16 bytes,
-    which int8_matmul reads fastest."""
+    """(codes of like's shape, distance of their rows): rows start at whole cache lines, which
+    int8_matmul reads fastest (777 x 5003 x 2050 at 2176 bytes a row 18.4 us, at 2064 20.3 us)."""
     shape = like.shape
     width = shape[-1]
-    stride = (width + 15) & ~15
+    stride = (width + 127) & ~127 if width > 128 else (width + 15) & ~15
     if stride == width:
         return _new(like, shape, torch.int8), width
     return _new(like, (*shape[:-1], stride), torch.int8)[..., :width], stride
@@ -125,8 +125,8 @@ def quantize_int8(x):
 
     scale = max|x| / 127, code = x / scale to the nearest, ties to even.  Rows of
     zeros have scale 0; rows with a NaN or an infinity have scale NaN and codes 0.
-    For weights a row is an output channel, for activations a token.  Rows of the
-    codes start at multiples of 16 bytes (codes.stride() says where).
+    For weights a row is an output channel, for activations a token.  Rows of more
+    than 128 codes start at multiples of 128 bytes (codes.stride() says where).
     """
     kind = _type_of(x, "x")
     _same_device(x)
@@ -179,7 +179,7 @@ def int8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
     b_scales float32 [N] (one for each output channel), as quantize_int8 gives them;
     bias float32 [N]; out of out_dtype (float32, bfloat16 or float16).  The sums are
     exact, so K is at most 131071; scales and bias are applied in 32 bits.  Rows of a
-    and b that start at multiples of 16 bytes are read fastest.
+    and b that start at multiples of 128 bytes are read fastest.
     """
     kind = _TYPE.get(out_dtype)
     if kind is None:
