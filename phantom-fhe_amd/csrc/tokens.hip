@@ -92,20 +92,27 @@ __device__ __forceinline__ void short_row_values(const RowArgs &a, const T *x, c
     }
 }
 
-// rint(v k): 1.5 2^52 leaves the sum's last bit at 1, so its low byte is the code, rounded
-// to nearest even.  In 64 bits, at the rate of 32: with k of 24 bits one value in 10^5 would
-// get the neighbouring code, and no k = 127 / top passes the range.
+// A code from the value and the factor, in the low byte.  The product is formed in 64 bits, at
+// the rate of 32: with a factor of 24 bits one value in 10^5 would get the neighbouring code, and
+// none passes the range.  The norm's is rounded at once (1.5 2^52 leaves the sum's last bit at
+// 1); quantization's first to the quotient in 32 bits, so that code is x / scale as any
+// program forms it.
+template <bool NORM>
 __device__ __forceinline__ uint32_t code_of(float v, double k) {
 #pragma clang fp contract(off)
     const double p = (double)v * k;
-    return (uint32_t)__double2loint(p + 6755399441055744.0);
+    if (NORM) return (uint32_t)__double2loint(p + 6755399441055744.0);
+    return __float_as_uint((float)p + 12582912.f);
 }
+template <bool NORM>
 __device__ __forceinline__ void store_codes(int8_t *codes, const float (&v)[kVec], double k, uint32_t keep) {
     uint32_t w[kVec / 4];
 #pragma unroll
     for (int e = 0; e < kVec; e += 4) {
-        const uint32_t lo = __builtin_amdgcn_perm(code_of(v[e + 1], k), code_of(v[e], k), 0x0c0c0400);
-        const uint32_t hi = __builtin_amdgcn_perm(code_of(v[e + 3], k), code_of(v[e + 2], k), 0x04000c0c);
+        uint32_t c[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) c[i] = code_of<NORM>(v[e + i], k);
+        const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0c);
         w[e / 4] = (lo | hi) & keep;
     }
     __builtin_memcpy(codes, w, kVec);
@@ -164,10 +171,12 @@ k_quantize_rows(RowArgs a) {
     }
     // a NaN, an infinity or a sum past float's range: a NaN scale, codes of 0
     const bool bad = s.top >= kInfBits || !(s.sum < __uint_as_float(kInfBits));
-    const double k = s.top == 0 ? 0. : 127. / (double)__uint_as_float(s.top);
+    const float top = __uint_as_float(s.top);
+    float scale = top * (1.f / 127.f);  // as a division by a constant is formed on the GPU
+    // the norm's scale has rsqrt() in it, and one that is nearly subnormal has few bits
+    const double k = s.top == 0 ? 0. : NORM || scale < 1e-30f ? 127. / (double)top : 1. / (double)scale;
     const uint32_t keep = bad ? 0u : ~0u;
     if (t == 0) {
-        float scale = __uint_as_float(s.top) / 127.f;
         if (NORM) scale *= rsqrtf(s.sum / (float)a.width + a.eps);
         a.scales[row] = bad ? __uint_as_float(0x7fc00000u) : scale;
     }
@@ -175,18 +184,18 @@ k_quantize_rows(RowArgs a) {
         if (t == 0)
 #pragma unroll
             for (int e = 0; e < kVec; e++)
-                if (e < (int)a.width) codes[e] = (int8_t)(code_of(v[0][e], k) & keep);
+                if (e < (int)a.width) codes[e] = (int8_t)(code_of<NORM>(v[0][e], k) & keep);
     } else if (STEPS) {
 #pragma unroll
         for (int j = 0; j < kHold; j++) {
             const uint32_t own = (j * THREADS + t) * kVec;
-            if (own < a.width) store_codes(codes + min(own, last), v[j], k, keep);
+            if (own < a.width) store_codes<NORM>(codes + min(own, last), v[j], k, keep);
         }
     } else {
         RowStat again{0.f, 0u};
         for (uint32_t own = t * kVec; own < a.width; own += THREADS * kVec) {
             row_values<T, NORM>(a, x, residual, nullptr, min(own, last), own, again, v[0]);
-            store_codes(codes + min(own, last), v[0], k, keep);
+            store_codes<NORM>(codes + min(own, last), v[0], k, keep);
         }
     }
 }
