@@ -201,6 +201,7 @@ k_tiles(MatmulArgs g) {
     auto landed = [&](bool more) {
         constexpr int kLeft = STAGES > 2 ? kLoads * (STAGES - 2) : 0;  // loads of the blocks behind it
         static_assert(kLeft < 64, "the counter's range");
+        asm volatile("" ::: "memory");
         if (more)
             __builtin_amdgcn_s_waitcnt(0x0070 | (kLeft & 15) | kLeft >> 4 << 14);
         else

@@ -177,7 +177,7 @@ k_quantize_rows(RowArgs a) {
     const double k = s.top == 0 ? 0. : NORM || scale < 1e-30f ? 127. / (double)top : 1. / (double)scale;
     const uint32_t keep = bad ? 0u : ~0u;
     if (t == 0) {
-        if (NORM) scale *= rsqrtf(s.sum / (float)a.width + a.eps);
+        if (NORM && s.top) scale *= rsqrtf(s.sum / (float)a.width + a.eps);  // 0 stays 0 at eps = 0
         a.scales[row] = bad ? __uint_as_float(0x7fc00000u) : scale;
     }
     if (brief) {
@@ -815,7 +815,7 @@ int pfa_token_probabilities(const void *logits, size_t stride, int type, size_t 
         require(!workspace_bytes || workspace, "null workspace");
         if (rows == 0 || vocab == 0) return;
         require(logits && out, "null argument");
-        require(apart(rows, stride, vocab), "rows overlap");
+        require(apart(rows, stride, vocab) && (!mask || apart(rows, mask_stride, vocab)), "rows overlap");
         aligned(logits, size, "logits");
         aligned(out, 4, "out");
         aligned(temperatures, 4, "temperatures");

@@ -124,6 +124,11 @@ def test_abi_refusals():
         ("pfa_token_probabilities", (p, 8, 0, 1, 8, None, -1.0, None, 0, p, None, 0, None), "temperature"),
         ("pfa_token_probabilities", (p, 8, 7, 1, 8, None, 1.0, None, 0, p, None, 0, None), "type"),
         ("pfa_token_probabilities", (p, 4, 0, 2, 8, None, 1.0, None, 0, p, None, 0, None), "overlap"),
+        ("pfa_token_probabilities", (p, 8, 0, 2, 8, None, 1.0, p, 4, p, None, 0, None), "overlap"),
+        ("pfa_token_probabilities", (p, 1 << 17, 0, 4, 1 << 17, None, 1.0, None, 0, p, None, 0, None), "workspace"),
+        ("pfa_verify_drafts", (p, 8, None, 4, 1, 1, 1 << 17, p, 1 << 18, 1 << 17, None, 0, 0, 0, p, p, 8, p, p, None, 0,
+                               None), "workspace"),
+        ("pfa_int8_matmul", (p, 16384, p, p, 16384, p, None, 64, 64, 16384, p, 0, 64, None, 0, None), "workspace"),
         ("pfa_token_probabilities", (None, 8, 0, 1, 8, None, 1.0, None, 0, p, None, 0, None), "null"),
         ("pfa_verify_drafts", (p, 2, None, 4, 1, 1, 8, p, 16, 8, None, 0, 0, 0, p, p, 8, p, p, None, 0, None), "bytes"),
         ("pfa_verify_drafts", (p, 8, p, 3, 1, 1, 8, p, 16, 8, None, 0, 0, 0, p, p, 8, p, p, None, 0, None), "bytes"),
@@ -145,6 +150,17 @@ def test_abi_empty_calls_launch_nothing():
     assert _abi("pfa_token_probabilities", None, 0, 0, 0, 5, None, 1.0, None, 0, None, None, 0, None)[0] == P.PFA_OK
     assert _abi("pfa_verify_drafts", None, 8, None, 4, 0, 0, 5, None, 0, 0, None, 0, 0, 0, None, None, 0, None, None,
                 None, 0, None)[0] == P.PFA_OK
+
+
+def test_workspace_sizes():
+    """What the calls need is what the queries say; short rows and large products need nothing."""
+    assert P.token_workspace(5, 131072) > 0 and P.token_workspace(1000, 8192) == 0
+    assert P.matmul_workspace(64, 64, 16384) % (64 * 64 * 4) == 0 and P.matmul_workspace(64, 64, 16384) > 0
+    assert P.matmul_workspace(4096, 16384, 4096) == 0 and P.matmul_workspace(1, 4096, 16384) == 0
+    for name, args in (("pfa_token_workspace", (1, 1)), ("pfa_matmul_workspace", (1, 1, 1))):
+        assert _abi(name, *args, None)[0] == P.PFA_ERR_INVALID_ARGUMENT
+    with pytest.raises(ValueError, match="131071"):
+        P.matmul_workspace(1, 1, 131072)
 
 
 def test_reference_closed_forms():

@@ -137,6 +137,8 @@ def test_norm_edges(dev):
         assert (codes[6:] == 127).all()
         # (2 / sqrt(4 + eps)) / 127
         assert (scales[6:] - 1 / 127).abs().max() < 1e-8
+        codes, scales, _ = ph.rms_norm_int8(x[:1] * 0, w, 0.0)  # nothing at all, not even eps
+        assert (codes == 0).all() and (scales == 0).all()
         w[3] = nan  # a gain that is no number reaches every row
         codes, scales, total = ph.rms_norm_int8(x, w, 1e-6, r)
         assert torch.isnan(scales).all() and (codes == 0).all()
