@@ -150,13 +150,15 @@ k_tiles(MatmulArgs g) {
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const uint32_t down = (g.M + BM - 1) / BM, across = (g.N + BN - 1) / BN;
     // workgroups are dealt to the 8 XCDs in turn: each XCD gets a run of tiles, in groups of
-    // 8 tiles of rows, so that its L2 holds what its tiles share
+    // some tiles of rows, so that its L2 holds what its tiles share (tiles of 256 rows, 8192 x
+    // 8192 x 4096, us: groups of 2, 4, 6, 8: 258, 266, 255, 266)
+    constexpr uint32_t kGroup = BM >= 256 ? 6 : 8;
     const uint32_t jobs = down * across * g.splits, each = (jobs + 7) / 8;
     const uint32_t job = blockIdx.x % 8 * each + blockIdx.x / 8;
     if (job >= jobs || blockIdx.x / 8 >= each) return;
     const uint32_t split = job % g.splits, t = job / g.splits;
-    const uint32_t group = t / (8 * across), height = min(8u, down - group * 8);
-    const uint32_t m0 = (group * 8 + t % (8 * across) % height) * BM, n0 = t % (8 * across) / height * BN;
+    const uint32_t group = t / (kGroup * across), height = min(kGroup, down - group * kGroup);
+    const uint32_t m0 = (group * kGroup + t % (kGroup * across) % height) * BM, n0 = t % (kGroup * across) / height * BN;
     const uint32_t wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
     // this workgroup's codes of K
     const uint32_t all = (g.K + kBlock - 1) / kBlock, share = (all + g.splits - 1) / g.splits;
@@ -371,10 +373,10 @@ struct Shape {
     uint32_t rows, cols;
     float alone, pair, each;
 };
-enum { kSmall, kSquare, kWide, kLarge, kBroad, kHuge, kShapes };
+enum { kSmall, kSquare, kWide, kLarge, kBroad, kHuge, kTall, kShapes };
 constexpr Shape shapes[kShapes] = {
     {32, 64, .19f, .25f, .12f}, {64, 64, .30f, .48f, .23f}, {64, 128, .47f, .70f, .35f},
-    {128, 128, .56f, 1.12f, .56f}, {128, 192, .66f, 1.32f, .66f}, {128, 256, .80f, 1.60f, .80f}};
+    {128, 128, .56f, 1.12f, .56f}, {128, 192, .66f, 1.32f, .66f}, {128, 256, .80f, 1.60f, .80f}, {256, 128, .80f, 1.55f, .76f}};
 
 // How a product is formed: `few` by k_few_rows, else by tiles of `shape`, K in `splits` parts.
 struct Plan {
@@ -442,7 +444,8 @@ void matmul(const MatmulArgs &g, const Plan &p, hipStream_t s) {
         case kWide: return launch_tiles<T, 16, 64, 128, 1, 4, 3>(g, s);
         case kLarge: return launch_tiles<T, 32, 128, 128, 2, 2, 3>(g, s);
         case kBroad: return launch_tiles<T, 16, 128, 192, 2, 4, 3>(g, s);
-        default: return launch_tiles<T, 16, 128, 256, 2, 4, 3>(g, s);
+        case kHuge: return launch_tiles<T, 16, 128, 256, 2, 4, 3>(g, s);
+        default: return launch_tiles<T, 16, 256, 128, 4, 2, 3>(g, s);
     }
 }
 

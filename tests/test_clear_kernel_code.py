@@ -31,7 +31,8 @@ def test_nothing_is_spilled(kernels):
 
 @pytest.mark.parametrize("shape,groups", [("16, 32, 64, 2, 2, 6", 2), ("16, 64, 64, 2, 2, 4", 2),
                                           ("16, 64, 128, 1, 4, 3", 2), ("32, 128, 128, 2, 2, 3", 1),
-                                          ("16, 128, 192, 2, 4, 3", 1), ("16, 128, 256, 2, 4, 3", 1)])
+                                          ("16, 128, 192, 2, 4, 3", 1), ("16, 128, 256, 2, 4, 3", 1),
+                                          ("16, 256, 128, 4, 2, 3", 1)])
 def test_tiles_fit(kernels, shape, groups):
     found = named(kernels, "k_tiles", shape)
     assert len(found) == 3  # the three types of outputs
