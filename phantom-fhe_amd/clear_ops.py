@@ -106,9 +106,14 @@ def _new_codes(like):
     shape = like.shape
     width = shape[-1]
     stride = (width + 127) & ~127 if width > 128 else (width + 15) & ~15
-    if stride == width:
+    if stride == width or not like.numel():
         return _new(like, shape, torch.int8), width
-    return _new(like, (*shape[:-1], stride), torch.int8)[..., :width], stride
+    strides, step = [1], stride
+    for n in shape[-2::-1]:
+        strides.append(step)
+        step *= n
+    # made with these strides at once: a view of whole rows would cost another 1.3 us
+    return torch.empty_strided(shape, strides[::-1], dtype=torch.int8, device=like.device), stride
 
 
 def _workspace(need, device):
@@ -132,8 +137,8 @@ def quantize_int8(x):
     _same_device(x)
     rows, stride = _matrix(x, "x")
     codes, codes_stride = _new_codes(x)
-    scales = _new(x, x.shape[:-1], torch.float32)
     n, width = rows.shape
+    scales = _new(x, (n,) if x.dim() == 2 else x.shape[:-1], torch.float32)
     if n:
         _call("pfa_quantize_int8", x, rows.data_ptr(), stride, kind, n, width, codes.data_ptr(), codes_stride,
               scales.data_ptr())
@@ -164,7 +169,7 @@ def rms_norm_int8(x, weight, eps=1e-6, residual=None):
         more, more_stride = _matrix(residual, "residual")
         total, total_stride = _new(x, x.shape, x.dtype), width
     codes, codes_stride = _new_codes(x)
-    scales = _new(x, x.shape[:-1], torch.float32)
+    scales = _new(x, (n,) if x.dim() == 2 else x.shape[:-1], torch.float32)
     if n:
         _call("pfa_rms_norm_int8", x, rows.data_ptr(), stride, more.data_ptr() if more is not None else None,
               more_stride, weight.data_ptr(), kind, n, width, float(eps), total.data_ptr() if total_stride else None,
@@ -281,9 +286,10 @@ def verify_drafts(draft_tokens, target_probs, uniforms, noise, draft_probs=None,
     drafts = places - 1
 
     def place(t, name):
-        if vocab > 1 and t.stride(2) != 1:
+        outer, step, inner = t.stride()
+        if inner != 1 and vocab > 1:
             _fail(f"{name}: the probabilities of a place must be adjacent")
-        return t.stride(0), t.stride(1)
+        return outer, step
 
     if draft_tokens.shape != (batch, drafts) or not draft_tokens.is_contiguous():
         _fail(f"draft_tokens: expected contiguous {(batch, drafts)}, got {tuple(draft_tokens.shape)}")
