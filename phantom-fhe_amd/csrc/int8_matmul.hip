@@ -120,7 +120,7 @@ k_few_rows(MatmulArgs g) {
 // 16, and chunk c of row r stands in place c ^ (r mod 8), so that a wave's reading of one
 // chunk of 8 rows touches every bank once.  MF is the matrix instruction: 32 x 32 outputs from 32
 // codes, or 16 x 16 from 64, whose shorter sums keep small tiles' chains short.  Large products
-// (4096 x 16384 x 4096: 252 us, 2.2 POP/s; 8192^3: 2.27) are bound by the blocks' way into the L2s, then by
+// (4096 x 16384 x 4096: 252 us, 8192^3: 460 us, 2.2 and 2.4 POP/s) are bound by the blocks' way into the L2s, then by
 // the matrix units (55 % busy); wide ones of few rows by reading b (20 x 131072 x 4096: 97 us, 5.6 TB/s);
 // small ones by the blocks' latency (128 x 4096 x 4096: 9.1 us).
 template <int MF>
