@@ -425,6 +425,11 @@ int pfa_rms_norm_int8(const void *x, size_t x_stride, const void *residual, size
 /* Bytes of workspace that pfa_int8_matmul needs for these sizes (0: none). */
 int pfa_matmul_workspace(size_t M, size_t N, size_t K, size_t *bytes);
 
+/* How pfa_int8_matmul forms a product of these sizes: tiles of tile_rows x tile_cols
+ * outputs with K in `splits` parts (tile_rows 0: few rows, b streamed 16 columns a
+ * workgroup).  Results do not depend on it; it says which kernel a size runs. */
+int pfa_matmul_plan(size_t M, size_t N, size_t K, size_t *tile_rows, size_t *tile_cols, size_t *splits);
+
 /* out[m][n] = (sum_k a[m][k] b[n][k]) a_scales[m] b_scales[n] + bias[n] (bias NULL:
  * none), out of `type`.  a [M][K], b [N][K].  The sums are exact: K <= 131071.
  * Rows of a and b that start at multiples of 128 bytes are read fastest.

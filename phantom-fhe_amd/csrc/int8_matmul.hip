@@ -471,6 +471,18 @@ int pfa_matmul_workspace(size_t M, size_t N, size_t K, size_t *bytes) {
     });
 }
 
+int pfa_matmul_plan(size_t M, size_t N, size_t K, size_t *tile_rows, size_t *tile_cols, size_t *splits) {
+    return guarded([&] {
+        require(tile_rows && tile_cols && splits, "null argument");
+        require(K <= kMostK, "pfa_matmul_plan: sums of more than 131071 products can pass 32 bits");
+        require(M <= 0x7fffffffu && N <= 0x7fffffffu, "pfa_matmul_plan: more than 2^31 - 1 rows");
+        const Plan p = plan_matmul(M, N, K);
+        *tile_rows = p.few ? 0 : shapes[p.shape].rows;
+        *tile_cols = p.few ? 16 : shapes[p.shape].cols;
+        *splits = p.splits;
+    });
+}
+
 int pfa_int8_matmul(const int8_t *a, size_t a_stride, const float *a_scales, const int8_t *b, size_t b_stride,
                     const float *b_scales, const float *bias, size_t M, size_t N, size_t K, void *out, int type,
                     size_t out_stride, void *workspace, size_t workspace_bytes, void *stream) {

@@ -79,6 +79,7 @@ SIGNATURES = {
     "pfa_quantize_int8": (_i32, [_vp, _sz, _i32, _sz, _sz, _vp, _sz, _vp, _vp]),
     "pfa_rms_norm_int8": (_i32, [_vp, _sz, _vp, _sz, _vp, _i32, _sz, _sz, C.c_double, _vp, _sz, _vp, _sz, _vp, _vp]),
     "pfa_matmul_workspace": (_i32, [_sz, _sz, _sz, C.POINTER(_sz)]),
+    "pfa_matmul_plan": (_i32, [_sz, _sz, _sz, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz)]),
     "pfa_int8_matmul": (_i32, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _i32, _sz, _vp, _sz, _vp]),
     "pfa_token_workspace": (_i32, [_sz, _sz, C.POINTER(_sz)]),
     "pfa_token_probabilities": (_i32, [_vp, _sz, _i32, _sz, _sz, _vp, C.c_double, _vp, _sz, _vp, _vp, _sz, _vp]),
@@ -199,6 +200,13 @@ def matmul_workspace(m: int, n: int, k: int) -> int:
     size = C.c_size_t(0)
     call("pfa_matmul_workspace", m, n, k, C.byref(size))
     return int(size.value)
+
+
+def matmul_plan(m: int, n: int, k: int) -> tuple[int, int, int]:
+    """(rows, columns, parts of K) of the tiles that form int8_matmul's outputs; rows 0: few rows, b streamed."""
+    out = [C.c_size_t(0) for _ in range(3)]
+    call("pfa_matmul_plan", m, n, k, *(C.byref(v) for v in out))
+    return tuple(int(v.value) for v in out)
 
 
 def galois_elt_from_step(step: int, poly_degree: int) -> int:
