@@ -415,9 +415,10 @@ int pfa_quantize_int8(const void *x, size_t x_stride, int type, size_t rows, siz
 
 /* y = x + residual (residual NULL: y = x), total = y rounded to `type` (written
  * only with a residual), then the codes and scales (as pfa_quantize_int8) of
- * y / sqrt(mean(y^2) + eps) * weight, from the unrounded y.  weight [width].  A
- * row whose sum of squares is not finite has scale NaN and codes 0.  total must not
- * overlap x or residual. */
+ * y / sqrt(mean(y^2) + eps) * weight, from the unrounded y.  weight [width].  y,
+ * y weight and the sum of squares are formed in 32 bits: a row where one of them is
+ * not finite there has scale NaN and codes 0.  Squares too small for 32 bits are not
+ * lost.  total must not overlap x or residual. */
 int pfa_rms_norm_int8(const void *x, size_t x_stride, const void *residual, size_t residual_stride,
                       const void *weight, int type, size_t rows, size_t width, double eps, void *total,
                       size_t total_stride, int8_t *codes, size_t codes_stride, float *scales, void *stream);

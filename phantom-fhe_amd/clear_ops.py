@@ -152,6 +152,8 @@ def rms_norm_int8(x, weight, eps=1e-6, residual=None):
     With y = x + residual: total = y in x's type (x itself without a residual), and
     codes, scales are quantize_int8's of y / sqrt(mean(y^2) + eps) * weight, formed from
     the unrounded y.  x [..., width]; residual like x; weight [width]; all of one type.
+    y, y weight and the sum of squares are formed in 32 bits: a row where one of them is
+    not finite there has scale NaN and codes 0.
     """
     kind = _type_of(x, "x")
     _same_device(x, weight, residual)

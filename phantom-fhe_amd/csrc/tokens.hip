@@ -39,7 +39,7 @@ struct RowArgs {
     float *scales;
     size_t rows, x_stride, residual_stride, total_stride, codes_stride;
     uint32_t width;
-    float eps;
+    double eps;
 };
 
 constexpr int kVec = 8;  // elements a thread takes at once: 16 bytes of the 2-byte types, 8 codes
@@ -90,6 +90,21 @@ __device__ __forceinline__ void short_row_values(const RowArgs &a, const T *x, c
             s.top = max(s.top, mag_bits(v[e]));
         }
     }
+}
+
+// Sum of squares of a row whose squares are lost in 32 bits, of values lifted by 2^100: in the
+// row's threads, to be added up.  Rare, so one place at a time.
+constexpr float kFewSquares = 0x1p-90f;
+template <class T>
+__device__ __forceinline__ float lifted_squares(const T *x, const T *residual, uint32_t width, uint32_t t,
+                                                uint32_t threads) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (uint32_t i = t; i < width; i += threads) {
+        const float y = ((float)x[i] + (residual ? (float)residual[i] : 0.f)) * 0x1p100f;
+        sum = fmaf(y, y, sum);
+    }
+    return sum;
 }
 
 // A code from the value and the factor, in the low byte.  The product is formed in 64 bits, at
@@ -177,8 +192,27 @@ k_quantize_rows(RowArgs a) {
     // the norm's scale has rsqrt() in it, and one that is nearly subnormal has few bits
     const double k = s.top == 0 ? 0. : NORM || scale < 1e-30f ? 127. / (double)top : 1. / (double)scale;
     const uint32_t keep = bad ? 0u : ~0u;
+    // Squares below 2^-126 lose bits, below 2^-149 all of them.  Where they could matter, in a sum below
+    // 2^-90 (2^30 of them make 2^-119) that eps does not outweigh, they are summed again.
+    float lifted = 0.f;
+    const bool few = NORM && s.top && s.sum < kFewSquares && a.eps < 0x1p-60;
+    if (few) {
+        lifted = wave_sum(lifted_squares(x, residual, a.width, t, THREADS));
+        if (!kWave) {
+            __shared__ float part[THREADS / 64];
+            if (t % 64 == 0) part[t / 64] = lifted;
+            __syncthreads();
+            lifted = 0.f;
+#pragma unroll
+            for (int w = 0; w < THREADS / 64; w++) lifted += part[w];
+        }
+    }
     if (t == 0) {
-        if (NORM && s.top) scale *= rsqrtf(s.sum / (float)a.width + a.eps);  // 0 stays 0 at eps = 0
+        if (NORM && s.top) {  // 0 stays 0 at eps = 0; the factor may be past 32 bits, and `top` subnormal
+            const double factor = few ? rsqrt((double)lifted * 0x1p-200 / a.width + a.eps)
+                                      : (double)rsqrtf(s.sum / (float)a.width + (float)a.eps);
+            scale = (float)((double)top * (1. / 127.) * factor);
+        }
         a.scales[row] = bad ? __uint_as_float(0x7fc00000u) : scale;
     }
     if (brief) {
@@ -802,7 +836,7 @@ int pfa_rms_norm_int8(const void *x, size_t x_stride, const void *residual, size
         aligned(total, size, "total");
         aligned(scales, 4, "scales");
         const RowArgs a{x,        residual,        weight,       total,        codes,           scales, rows,
-                        x_stride, residual_stride, total_stride, codes_stride, (uint32_t)width, (float)eps};
+                        x_stride, residual_stride, total_stride, codes_stride, (uint32_t)width, eps};
         with_type(type, [&](auto t) { quantize_rows<decltype(t), true>(a, as_stream(stream)); });
         PFA_HIP(hipGetLastError());
     });

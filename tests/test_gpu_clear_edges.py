@@ -1,0 +1,38 @@
+"""Where the clear operators' 32 bits end, and the rules of their roundings, against the definitions."""
+import numpy as np
+import pytest
+
+import clear_reference as R
+import pyPhantom as ph
+from test_gpu_clear_ops import check_codes, dtype_of, f64, layouts, normal
+
+pytestmark = pytest.mark.gpu
+
+# reaches every kernel of the rows: a wave with and without whole vectors, 256 and 1024 threads, rows read twice
+WIDTHS = [1, 5, 9, 300, 2047, 4096, 8190, 16384, 20003, 32770, 40001, 70000]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_norm_of_tiny_rows(dev, dtype, width):
+    """Squares that are subnormal or vanish in 32 bits, at an eps that does not hide them, beside ordinary rows."""
+    import torch
+
+    x, r = (normal(width + k, 7, width, dtype="float32", dev=dev, spread=0.1) for k in (0, 1))
+    size = torch.tensor([1e-23, 1.0, 1e-30, 0.0, 1e-19, 1e-14, 1e-36], device=dev)[:, None]
+    x, r = ((t * size).to(dtype_of(dtype)) for t in (x, r))
+    w = normal(3, width, dtype=dtype, dev=dev, spread=0.1)
+    for eps in (0.0, 1e-60, 1e-30):
+        for res in (None, r):
+            codes, scales, total = ph.rms_norm_int8(layouts(x, "odd"), w, eps, res)
+            with np.errstate(all="ignore"):
+                v = R.rms_norm(f64(x), f64(w), eps, None if res is None else f64(res))
+            v[3] = 0  # a row of zeros
+            check_codes(codes, scales, v, width / 64 + 20)
+    # the smallest numbers there are
+    whole = torch.randint(-900, 901, (3, width), generator=torch.Generator().manual_seed(width)).to(dev)
+    whole[:, 0] = 900
+    x = (whole.double() * 2.0 ** (-149 if dtype == "float32" else -133)).to(dtype_of(dtype))
+    one = torch.ones(width, device=dev, dtype=x.dtype)
+    codes, scales, _ = ph.rms_norm_int8(x, one, 0.0)
+    check_codes(codes, scales, R.rms_norm(f64(x), f64(one), 0.0), width / 64 + 20)
