@@ -407,9 +407,10 @@ int pfa_ct_lincomb(const pfa_context *ctx, size_t L, size_t size, size_t ct_size
 #define PFA_BF16 1
 #define PFA_F16 2
 
-/* Rows of x [rows][width] as codes of 8 bits: scale = max|x| / 127, code =
- * x / scale rounded to the nearest integer, ties to even.  A row of zeros has
- * scale 0 and codes 0; a row with a NaN or an infinity has scale NaN and codes 0. */
+/* Rows of x [rows][width] as codes of 8 bits: scale = max|x| / 127, rounded to 32
+ * bits, code = 127 x / max|x| to the nearest integer, ties to even.  A row of zeros
+ * has scale 0 and codes 0 (one so small that only its scale rounds to 0 keeps its
+ * codes); a row with a NaN or an infinity has scale NaN and codes 0. */
 int pfa_quantize_int8(const void *x, size_t x_stride, int type, size_t rows, size_t width, int8_t *codes,
                       size_t codes_stride, float *scales, void *stream);
 
@@ -417,7 +418,8 @@ int pfa_quantize_int8(const void *x, size_t x_stride, int type, size_t rows, siz
  * only with a residual), then the codes and scales (as pfa_quantize_int8) of
  * y / sqrt(mean(y^2) + eps) * weight, from the unrounded y.  weight [width].  y,
  * y weight and the sum of squares are formed in 32 bits: a row where one of them is
- * not finite there has scale NaN and codes 0.  Squares too small for 32 bits are not
+ * not finite there has scale NaN and codes 0.  The codes are those of y weight (the
+ * root is common to a row and changes none).  Squares too small for 32 bits are not
  * lost.  total must not overlap x or residual. */
 int pfa_rms_norm_int8(const void *x, size_t x_stride, const void *residual, size_t residual_stride,
                       const void *weight, int type, size_t rows, size_t width, double eps, void *total,

@@ -128,9 +128,9 @@ def quantize_int8(x):
     """Codes of 8 bits of x [..., width], with one scale for each row: (codes int8
     [..., width], scales float32 [...]), x ~ codes * scales.
 
-    scale = max|x| / 127, code = x / scale to the nearest, ties to even.  Rows of
-    zeros have scale 0; rows with a NaN or an infinity have scale NaN and codes 0.
-    For weights a row is an output channel, for activations a token.  Rows of more
+    scale = max|x| / 127, rounded to 32 bits, code = 127 x / max|x| to the nearest, ties
+    to even.  Rows of zeros have scale 0 (one so small that only its scale rounds to 0
+    keeps its codes); rows with a NaN or an infinity have scale NaN and codes 0.  For weights a row is an output channel, for activations a token.  Rows of more
     than 128 codes start at multiples of 128 bytes (codes.stride() says where).
     """
     kind = _type_of(x, "x")
@@ -153,7 +153,8 @@ def rms_norm_int8(x, weight, eps=1e-6, residual=None):
     codes, scales are quantize_int8's of y / sqrt(mean(y^2) + eps) * weight, formed from
     the unrounded y.  x [..., width]; residual like x; weight [width]; all of one type.
     y, y weight and the sum of squares are formed in 32 bits: a row where one of them is
-    not finite there has scale NaN and codes 0.
+    not finite there has scale NaN and codes 0.  The codes are those of y weight (the
+    root is common to a row and changes none).
     """
     kind = _type_of(x, "x")
     _same_device(x, weight, residual)

@@ -22,7 +22,7 @@ dim3 row_grid(size_t rows) {
     return dim3((uint32_t)std::min<size_t>(rows, kRowsX), (uint32_t)((rows + kRowsX - 1) / kRowsX));
 }
 
-// Codes of one row.  With k = 127 / max|v| every code is rint(v k); the norm's
+// Codes of one row: 127 v / max|v| to the nearest; the norm's
 // factor rsqrt(mean + eps) is common to the row and cancels, so the sum of
 // squares and the maximum come from the same pass.  4096 x 8192 of bf16 with a
 // residual: 45 us (235 MB, 5.2 TB/s); 2048 x 16384 quantized: 17.4 us (5.8 TB/s);
@@ -107,26 +107,21 @@ __device__ __forceinline__ float lifted_squares(const T *x, const T *residual, u
     return sum;
 }
 
-// A code from the value and the factor, in the low byte.  The product is formed in 64 bits, at
-// the rate of 32: with a factor of 24 bits one value in 10^5 would get the neighbouring code, and
-// none passes the range.  The norm's is rounded at once (1.5 2^52 leaves the sum's last bit at
-// 1); quantization's first to the quotient in 32 bits, so that code is x / scale as any
-// program forms it.
-template <bool NORM>
+// A code from the value and k = 127 / max|v|, in the low byte: 127 v / max|v| to the nearest, ties to
+// even, for every v.  What is no tie is 2^-33 or more from one (v and max|v| have 24 bits), and k's
+// rounding moves a product by 2^-46: rounded at 2^-40 (the unit of 6144), ties are ties again, and 1.5 2^52
+// then leaves the code in the sum's last bits.  Two operations of 64 bits, at the rate of 32; with a factor of
+// 24 bits one value in 10^5 would get the neighbouring code.
 __device__ __forceinline__ uint32_t code_of(float v, double k) {
-#pragma clang fp contract(off)
-    const double p = (double)v * k;
-    if (NORM) return (uint32_t)__double2loint(p + 6755399441055744.0);
-    return __float_as_uint((float)p + 12582912.f);
+    return (uint32_t)__double2loint(fma((double)v, k, 6144.) + (6755399441055744. - 6144.));
 }
-template <bool NORM>
 __device__ __forceinline__ void store_codes(int8_t *codes, const float (&v)[kVec], double k, uint32_t keep) {
     uint32_t w[kVec / 4];
 #pragma unroll
     for (int e = 0; e < kVec; e += 4) {
         uint32_t c[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) c[i] = code_of<NORM>(v[e + i], k);
+        for (int i = 0; i < 4; i++) c[i] = code_of(v[e + i], k);
         const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0c);
         w[e / 4] = (lo | hi) & keep;
     }
@@ -188,10 +183,27 @@ k_quantize_rows(RowArgs a) {
     // a NaN, an infinity or a sum past float's range: a NaN scale, codes of 0
     const bool bad = s.top >= kInfBits || !(s.sum < __uint_as_float(kInfBits));
     const float top = __uint_as_float(s.top);
-    float scale = top * (1.f / 127.f);  // as a division by a constant is formed on the GPU
-    // the norm's scale has rsqrt() in it, and one that is nearly subnormal has few bits
-    const double k = s.top == 0 ? 0. : NORM || scale < 1e-30f ? 127. / (double)top : 1. / (double)scale;
+    const double k = s.top ? 127. / (double)top : 0.;
     const uint32_t keep = bad ? 0u : ~0u;
+    if (brief) {
+        if (t == 0)
+#pragma unroll
+            for (int e = 0; e < kVec; e++)
+                if (e < (int)a.width) codes[e] = (int8_t)(code_of(v[0][e], k) & keep);
+    } else if (STEPS) {
+#pragma unroll
+        for (int j = 0; j < kHold; j++) {
+            const uint32_t own = (j * THREADS + t) * kVec;
+            if (own < a.width) store_codes(codes + min(own, last), v[j], k, keep);
+        }
+    } else {
+        RowStat again{0.f, 0u};
+        for (uint32_t own = t * kVec; own < a.width; own += THREADS * kVec) {
+            row_values<T, NORM>(a, x, residual, nullptr, min(own, last), own, again, v[0]);
+            store_codes(codes + min(own, last), v[0], k, keep);
+        }
+    }
+    // The scale, behind the codes, which do not wait for it (in front 4096 x 8192 took 0.5 us more).
     // Squares below 2^-126 lose bits, below 2^-149 all of them.  Where they could matter, in a sum below
     // 2^-90 (2^30 of them make 2^-119) that eps does not outweigh, they are summed again.
     float lifted = 0.f;
@@ -208,30 +220,13 @@ k_quantize_rows(RowArgs a) {
         }
     }
     if (t == 0) {
+        float scale = top / 127.f;
         if (NORM && s.top) {  // 0 stays 0 at eps = 0; the factor may be past 32 bits, and `top` subnormal
             const double factor = few ? rsqrt((double)lifted * 0x1p-200 / a.width + a.eps)
                                       : (double)rsqrtf(s.sum / (float)a.width + (float)a.eps);
             scale = (float)((double)top * (1. / 127.) * factor);
         }
         a.scales[row] = bad ? __uint_as_float(0x7fc00000u) : scale;
-    }
-    if (brief) {
-        if (t == 0)
-#pragma unroll
-            for (int e = 0; e < kVec; e++)
-                if (e < (int)a.width) codes[e] = (int8_t)(code_of<NORM>(v[0][e], k) & keep);
-    } else if (STEPS) {
-#pragma unroll
-        for (int j = 0; j < kHold; j++) {
-            const uint32_t own = (j * THREADS + t) * kVec;
-            if (own < a.width) store_codes<NORM>(codes + min(own, last), v[j], k, keep);
-        }
-    } else {
-        RowStat again{0.f, 0u};
-        for (uint32_t own = t * kVec; own < a.width; own += THREADS * kVec) {
-            row_values<T, NORM>(a, x, residual, nullptr, min(own, last), own, again, v[0]);
-            store_codes<NORM>(codes + min(own, last), v[0], k, keep);
-        }
     }
 }
 

@@ -4,7 +4,7 @@ import pytest
 
 import clear_reference as R
 import pyPhantom as ph
-from test_gpu_clear_ops import check_codes, dtype_of, f64, layouts, normal
+from test_gpu_clear_ops import TYPES, check_codes, dtype_of, f64, layouts, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +36,45 @@ def test_norm_of_tiny_rows(dev, dtype, width):
     one = torch.ones(width, device=dev, dtype=x.dtype)
     codes, scales, _ = ph.rms_norm_int8(x, one, 0.0)
     check_codes(codes, scales, R.rms_norm(f64(x), f64(one), 0.0), width / 64 + 20)
+
+
+def nearest(codes, v):
+    """codes are 127 v / max|v| to the nearest, ties to even: exact in 64 bits (127 v and code max|v| have 31 bits)."""
+    c, v = codes.double(), v.double()
+    top = v.abs().amax(-1, keepdim=True)
+    off = (127 * v - c * top).abs() * 2
+    return bool(((off < top) | ((off == top) & (c % 2 == 0))).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", WIDTHS)
+def test_codes_are_the_nearest(dev, dtype, width):
+    """Every code and every scale by the definition, bit for bit: many values, and many that stand on a tie (half the
+    largest one is 63.5 steps)."""
+    import torch
+
+    rows = max(8, (1 << 21) // width)
+    x = normal(width, rows, width, dtype=dtype, dev=dev, spread=0.2)
+    top = x.abs().amax(-1)
+    x[:, width // 2::5] = (top / 2)[:, None]
+    x[::2, width // 3::7] = (-top / 2)[::2, None]
+    x[:, 0] = top
+    codes, scales = ph.quantize_int8(x)
+    assert nearest(codes, x)
+    # a quotient of 24 bits rounded from 53 is the one rounded at once
+    assert torch.equal(scales, (x.double().abs().amax(-1) / 127).float())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", WIDTHS)
+def test_norm_has_the_quantizations_codes(dev, dtype, width):
+    """The norm's factor is common to a row: its codes are those of (x + residual) weight, each rounded to 32 bits."""
+    import torch
+
+    rows = max(8, (1 << 21) // width)
+    x, r = (normal(width + k, rows, width, dtype=dtype, dev=dev, spread=0.2) for k in (0, 1))
+    w = normal(width, width, dtype=dtype, dev=dev, spread=0.2)
+    codes, _, _ = ph.rms_norm_int8(x, w, 1e-6, r)
+    y = (x.float() + r.float()) * w.float()
+    assert torch.equal(codes, ph.quantize_int8(y)[0])
+    assert nearest(codes, y)
