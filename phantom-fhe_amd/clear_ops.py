@@ -158,8 +158,8 @@ def rms_norm_int8(x, weight, eps=1e-6, residual=None):
     """
     kind = _type_of(x, "x")
     _same_device(x, weight, residual)
-    if not eps >= 0:
-        _fail("eps must be 0 or more")
+    if not 0 <= eps < float("inf"):
+        _fail("eps must be finite and 0 or more")
     rows, stride = _matrix(x, "x")
     n, width = rows.shape
     if width == 0:
@@ -237,7 +237,7 @@ def token_probabilities(logits, temperature=1.0, mask=None):
     else:
         one = float(temperature)
         if not 0 <= one < float("inf"):
-            _fail("the temperature must be 0 or more")
+            _fail("the temperature must be finite and 0 or more")
     allowed, mask_stride = None, 0
     if mask is not None:
         if mask.dtype != torch.bool or (mask.shape != logits.shape and mask.shape != (vocab,)):

@@ -6,6 +6,7 @@
 // All of them are bound by memory: a few operations for each element that is
 // read.  Statistics are held in 32 bits throughout.
 #include <algorithm>
+#include <cmath>
 
 #include "element.h"
 
@@ -222,8 +223,9 @@ k_quantize_rows(RowArgs a) {
     if (t == 0) {
         float scale = top / 127.f;
         if (NORM && s.top) {  // 0 stays 0 at eps = 0; the factor may be past 32 bits, and `top` subnormal
-            const double factor = few ? rsqrt((double)lifted * 0x1p-200 / a.width + a.eps)
-                                      : (double)rsqrtf(s.sum / (float)a.width + (float)a.eps);
+            const double sum = few ? (double)lifted * 0x1p-200 : (double)s.sum;
+            const double factor = few || a.eps > 0x1p100 ? rsqrt(sum / a.width + a.eps)
+                                                         : (double)rsqrtf(s.sum / (float)a.width + (float)a.eps);
             scale = (float)((double)top * (1. / 127.) * factor);
         }
         a.scales[row] = bad ? __uint_as_float(0x7fc00000u) : scale;
@@ -817,7 +819,7 @@ int pfa_rms_norm_int8(const void *x, size_t x_stride, const void *residual, size
     return guarded([&] {
         const size_t size = type_bytes(type);
         check_rows(rows, width, "pfa_rms_norm_int8");
-        require(eps >= 0 && eps <= 1e30, "pfa_rms_norm_int8: eps must be 0 or more");
+        require(eps >= 0 && eps < INFINITY, "pfa_rms_norm_int8: eps must be finite and 0 or more");
         if (rows == 0) return;
         require(width >= 1, "pfa_rms_norm_int8: the mean of an empty row");
         require(x && weight && codes && scales && (!residual || total), "null argument");
@@ -843,8 +845,7 @@ int pfa_token_probabilities(const void *logits, size_t stride, int type, size_t 
     return guarded([&] {
         const size_t size = type_bytes(type);
         check_rows(rows, vocab, "pfa_token_probabilities");
-        require(temperatures || (temperature >= 0 && temperature <= 1e30),
-                "pfa_token_probabilities: the temperature must be 0 or more");
+        require(temperatures || temperature >= 0, "pfa_token_probabilities: the temperature must be 0 or more");
         require(!workspace_bytes || workspace, "null workspace");
         if (rows == 0 || vocab == 0) return;
         require(logits && out, "null argument");

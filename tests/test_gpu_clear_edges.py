@@ -4,7 +4,7 @@ import pytest
 
 import clear_reference as R
 import pyPhantom as ph
-from test_gpu_clear_ops import TYPES, check_codes, dtype_of, f64, layouts, normal
+from test_gpu_clear_ops import TYPES, check_codes, check_probs, dtype_of, f64, layouts, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,25 @@ def test_norm_has_the_quantizations_codes(dev, dtype, width):
     y = (x.float() + r.float()) * w.float()
     assert torch.equal(codes, ph.quantize_int8(y)[0])
     assert nearest(codes, y)
+
+
+@pytest.mark.parametrize("heat", [1e31, 1e38])
+def test_large_temperatures(dev, heat):
+    """A number means what a tensor of it means, up to the largest."""
+    import torch
+
+    x = normal(1, 4, 300, dev=dev) * 1e30
+    p = ph.token_probabilities(x, heat)
+    assert torch.equal(p, ph.token_probabilities(x, torch.full((4,), heat, device=dev)))
+    check_probs(p, f64(x), np.full(4, float(np.float32(heat))), None)
+
+
+@pytest.mark.parametrize("eps", [1e31, 1e39, 1e60])
+def test_large_eps(dev, eps):
+    """An eps past 32 bits leaves scales within them."""
+    for width in (5, 300, 4096, 40001):
+        x = normal(width, 3, width, dev=dev, spread=0.1) * 1e15
+        w = normal(1, width, dev=dev, spread=0.1)
+        codes, scales, _ = ph.rms_norm_int8(x, w, eps)
+        assert (scales > 0).all()
+        check_codes(codes, scales, R.rms_norm(f64(x), f64(w), eps), width / 64 + 20)
