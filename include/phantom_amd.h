@@ -450,7 +450,8 @@ int pfa_token_workspace(size_t rows, size_t vocab, size_t *bytes);
  * temperature) over the places where mask [rows][vocab] (bytes; mask_stride 0:
  * one row for all; NULL: everywhere) is not 0; 0 elsewhere, whatever stands
  * there.  A row's temperature is temperatures[row], or `temperature` where
- * temperatures is NULL; at 0 the lowest place of the largest logit gets 1.  A row
+ * temperatures is NULL, in 32 bits; at 0 the lowest place of the largest logit gets
+ * 1, at +infinity all finite logits the same.  A row
  * that allows nothing, or -infinity alone, is all 0.  A NaN or (above temperature
  * 0) +infinity in an allowed place, or a negative or NaN temperature, makes the
  * row's allowed places NaN.  workspace: pfa_token_workspace bytes, otherwise as in

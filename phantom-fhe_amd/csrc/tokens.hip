@@ -253,7 +253,7 @@ void quantize_rows(const RowArgs &a, hipStream_t s) {
     launch_rows<T, NORM, 1024, 0>(a, s);
 }
 
-// Probabilities of one row: exp2((l - m) c) / sum, c = log2(e) / temperature, m the
+// Probabilities of one row: exp2((l - m) / 2 c) / sum, c = 2 log2(e) / temperature, m the
 // largest allowed logit; temperature 0 leaves the lowest place of m alone.
 struct ProbArgs {
     const void *logits;
@@ -270,12 +270,13 @@ constexpr float kLog2e = 1.44269504088896341f;
 __device__ __forceinline__ float infinity() { return __uint_as_float(kInfBits); }
 __device__ __forceinline__ float not_a_number() { return __uint_as_float(0x7fc00000u); }
 
-// log2(e) / t within float's range: a subnormal t must not make 0 c a NaN
-__device__ __forceinline__ float rate_of(float t) { return fminf(kLog2e / t, 3e38f); }
+// 2 log2(e) / t within float's range: a subnormal t must not make 0 c a NaN
+__device__ __forceinline__ float rate_of(float t) { return fminf(2.f * kLog2e / t, 3e38f); }
 
-// e^((l - m) / t).  The bound takes -infinity (also at an infinite t) to 0; m is finite.
+// e^((l - m) / t).  The difference is formed halved, as one of two numbers of 32 bits may pass them and an
+// infinite or large t brings it back.  The bound takes -infinity (also at an infinite t) to 0; m is finite.
 __device__ __forceinline__ float weight_of(float l, float m, float c) {
-    return __builtin_amdgcn_exp2f(fmaxf((l - m) * c, -200.f));
+    return __builtin_amdgcn_exp2f(fmaxf(fmaf(l, 0.5f, -0.5f * m) * c, -200.f));
 }
 
 // kVec logits from i on, -infinity where no token is allowed or the place is before `own`
@@ -344,7 +345,18 @@ struct ProbRow {
                 sum += v[j][e];
             }
         __shared__ float part[THREADS / 64];
-        sum = wave_sum(sum);
+        if (THREADS == 1024) {
+            // as wave_sum, but the lanes' addresses are formed anew: kept since share_top they push a row's values
+            // out of its 64 registers, and back on the way to the sum (320 rows of 32768 20.3 us, kept 21.1; rows of
+            // 256 threads have room: 2000 of 5003 15.5 us, anew 15.8)
+            uint32_t lane = threadIdx.x;
+            asm volatile("" : "+v"(lane));
+#pragma unroll
+            for (uint32_t d = 32; d; d >>= 1)
+                sum += __int_as_float(__builtin_amdgcn_ds_bpermute((int)((lane ^ d) * 4), __float_as_int(sum)));
+        } else {
+            sum = wave_sum(sum);
+        }
         if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = sum;
         __syncthreads();
         sum = part[0];

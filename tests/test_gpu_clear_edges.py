@@ -1,4 +1,6 @@
 """Where the clear operators' 32 bits end, and the rules of their roundings, against the definitions."""
+import math
+
 import numpy as np
 import pytest
 
@@ -100,3 +102,21 @@ def test_large_eps(dev, eps):
         codes, scales, _ = ph.rms_norm_int8(x, w, eps)
         assert (scales > 0).all()
         check_codes(codes, scales, R.rms_norm(f64(x), f64(w), eps), width / 64 + 20)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,vocab", [(4, 5), (4, 300), (4, 9000), (70, 20000), (4, 131072)])
+def test_logits_of_the_types_range(dev, dtype, rows, vocab):
+    """Differences of logits that pass 32 bits, at temperatures that bring them back, the infinite one among them."""
+    import torch
+
+    x = (normal(vocab, rows, vocab, spread=0) * 1e38).clamp_(-3.3e38, 3.3e38)
+    x[:, 0], x[:, -1] = 3.3e38, -3.3e38
+    x = x.to(dtype_of(dtype))
+    mask = torch.rand((rows, vocab), generator=torch.Generator().manual_seed(1)) < 0.5
+    mask[:, 0] = mask[:, -1] = True
+    for heat in (1e37, 1e38, 2e38, math.inf):
+        t = torch.full((rows,), heat)
+        for m in (None, mask):
+            p = ph.token_probabilities(x.to(dev), t.to(dev), None if m is None else m.to(dev))
+            check_probs(p, f64(x), f64(t), None if m is None else m.numpy())
