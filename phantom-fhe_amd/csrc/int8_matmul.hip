@@ -5,7 +5,6 @@
 // are applied in 32-bit floats, and one rounding leads to the output's type.
 #include <algorithm>
 #include <cmath>
-#include <mutex>
 #include <type_traits>
 
 #include "element.h"
@@ -149,7 +148,17 @@ k_tiles(MatmulArgs g) {
     constexpr int kLanes = 64 / MF;            // lanes that share a row of a fragment
     static_assert(kRows % (8 * WAVES) == 0 && BM % 8 == 0, "whole loads");
     using M = Matrix<MF>;
-    extern __shared__ __align__(1024) int8_t ring[];
+    // The ring, and in its place behind the products the scales, offsets and a line of outputs a wave.  Part of the
+    // kernel and not of the launch, where more than 64 KiB need a limit raised on every device.
+    constexpr int kRing = kStage * STAGES, kLines = (BN * 2 + BM) * 4 + WAVES * MF * (BN / WN * 4 + 16);
+    constexpr int kLds = kRing > kLines ? kRing : kLines;
+    static_assert(kLds <= 160 * 1024, "a CU's LDS");
+    __shared__ __align__(1024) int8_t held[kLds];
+    // where it begins is not told to the compiler: the tile of 32 x 64 then moves its sums from one register to
+    // another in every block (17 x 4096 x 4096 8.9 us, told 9.4)
+    uint32_t start = 0;
+    asm("" : "+s"(start));
+    int8_t *ring = held + start;
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const uint32_t down = (g.M + BM - 1) / BM, across = (g.N + BN - 1) / BN;
     // workgroups are dealt to the 8 XCDs in turn: each XCD gets a run of tiles, in groups of
@@ -420,18 +429,10 @@ Plan plan_matmul(size_t M, size_t N, size_t K) {
 
 template <class T, int MF, int BM, int BN, int WM, int WN, int STAGES>
 void launch_tiles(const MatmulArgs &g, hipStream_t s) {
-    constexpr size_t ring = (size_t)(BM + BN) * kBlock * STAGES;
-    constexpr size_t lines = (BN * 2 + BM) * 4 + WM * WN * MF * (BN / WN * 4 + 16);
-    constexpr size_t lds = ring > lines ? ring : lines;
-    static_assert(lds <= 160 * 1024, "a CU's LDS");
     const auto kernel = &k_tiles<T, MF, BM, BN, WM, WN, STAGES>;
-    static std::once_flag once;  // the attribute holds for every device
-    std::call_once(once, [&] {
-        PFA_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    });
     const size_t jobs = (size_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN) * g.splits;
     require(jobs < 1u << 22, "pfa_int8_matmul: more outputs than one launch can form");
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)((jobs + 7) / 8 * 8)), dim3(WM * WN * 64), lds, s, g);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)((jobs + 7) / 8 * 8)), dim3(WM * WN * 64), 0, s, g);
     if (g.splits > 1)
         hipLaunchKernelGGL(k_join<T>, dim3((uint32_t)(((size_t)g.M * ((g.N + 3) / 4) + 255) / 256)), dim3(256), 0, s, g);
 }
