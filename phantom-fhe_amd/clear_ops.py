@@ -8,9 +8,12 @@ pass takes so long that several drafted tokens are checked per pass).  Callers u
 them through pyPhantom, which re-exports them.
 
 They take torch tensors on a GPU, launch on torch's current stream of the tensors'
-device, return new tensors and never wait for the GPU.  Rows may be strided, the
-elements of a row are adjacent.  Wrong arguments raise ValueError, as everywhere in
-pyPhantom.  There is no CPU fallback.
+device, return new tensors (rms_norm_int8 without a residual returns x itself as the
+total) and never wait for the GPU.  Rows may be strided, the elements of a row are
+adjacent.  Wrong arguments raise ValueError, as everywhere in pyPhantom.  They are for
+inference: what they return carries no gradient, whatever its inputs require, and
+they take real tensors only, not those of torch's tracing or vmap.  There is no CPU
+fallback.
 """
 from __future__ import annotations
 

@@ -23,11 +23,8 @@ dim3 row_grid(size_t rows) {
     return dim3((uint32_t)std::min<size_t>(rows, kRowsX), (uint32_t)((rows + kRowsX - 1) / kRowsX));
 }
 
-// Codes of one row: 127 v / max|v| to the nearest; the norm's
-// factor rsqrt(mean + eps) is common to the row and cancels, so the sum of
-// squares and the maximum come from the same pass.  4096 x 8192 of bf16 with a
-// residual: 45 us (235 MB, 5.2 TB/s); 2048 x 16384 quantized: 17.4 us (5.8 TB/s);
-// one row of 4096: 3.1 us.
+// Codes of one row: 127 v / max|v| to the nearest.  The norm's factor rsqrt(mean + eps) is
+// common to the row and cancels, so the sum of squares and the maximum come from the same pass.
 struct RowStat {
     float sum;     // of squares
     uint32_t top;  // largest |y w|, as mag_bits
@@ -134,8 +131,9 @@ __device__ __forceinline__ void store_codes(int8_t *codes, const float (&v)[kVec
 // width is no multiple of kVec (its vector then starts early, and threads past the end
 // read it too), so no load stands behind a branch and all of them are in flight at once.
 // THREADS = 64: four rows a workgroup, one a wave, no barrier.  STEPS = 0: rows too
-// long for the registers are read twice.  Bound by memory: 2048 x 16384 bf16 in 18.2 us (5.5 TB/s),
-// with norm and residual 4096 x 8192 in 45.5 us (5.2 TB/s).
+// long for the registers are read twice.  Bound by memory: 2048 x 16384 bf16 in 18.2 us (5.5 TB/s), float32 29 us
+// (5.8 TB/s); with norm and residual 4096 x 8192 bf16 in 46 us (5.1 TB/s), float32 83 us (5.2 TB/s); one row of
+// 4096 in 3.1 us, a launch and one trip to memory.
 template <class T, bool NORM, int THREADS, int STEPS>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
 k_quantize_rows(RowArgs a) {
@@ -392,7 +390,7 @@ __device__ __forceinline__ void write_nan(const uint8_t *mask, float *out, uint3
 
 // Rows in one piece: read once, reduced twice, written once.  Two workgroups of 1024
 // threads on a CU (64 registers a lane) let one read while the other writes: 4096 rows of
-// 32768 bf16 in 167 us (4.8 TB/s), with one of them 203 us.
+// 32768 bf16 in 166 us (4.8 TB/s), with one of them 203 us.
 template <class T, int THREADS, int STEPS>
 __global__ void __launch_bounds__(THREADS, THREADS == 1024 && STEPS <= 4 ? 8 : 1)
 k_prob_rows(ProbArgs a) {
