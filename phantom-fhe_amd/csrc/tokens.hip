@@ -251,7 +251,7 @@ void quantize_rows(const RowArgs &a, hipStream_t s) {
     launch_rows<T, NORM, 1024, 0>(a, s);
 }
 
-// Probabilities of one row: exp2((l - m) / 2 c) / sum, c = 2 log2(e) / temperature, m the
+// Probabilities of one row: exp2((l - m) log2(e) / temperature) / sum, m the
 // largest allowed logit; temperature 0 leaves the lowest place of m alone.
 struct ProbArgs {
     const void *logits;
@@ -268,14 +268,20 @@ constexpr float kLog2e = 1.44269504088896341f;
 __device__ __forceinline__ float infinity() { return __uint_as_float(kInfBits); }
 __device__ __forceinline__ float not_a_number() { return __uint_as_float(0x7fc00000u); }
 
-// 2 log2(e) / t within float's range: a subnormal t must not make 0 c a NaN
-__device__ __forceinline__ float rate_of(float t) { return fminf(2.f * kLog2e / t, 3e38f); }
-
-// e^((l - m) / t).  The difference is formed halved, as one of two numbers of 32 bits may pass them and an
-// infinite or large t brings it back.  The bound takes -infinity (also at an infinite t) to 0; m is finite.
-__device__ __forceinline__ float weight_of(float l, float m, float c) {
-    return __builtin_amdgcn_exp2f(fmaxf(fmaf(l, 0.5f, -0.5f * m) * c, -200.f));
-}
+// e^((l - m) / t) = exp2((half l - half m) rate).  From t = 1 on the difference is formed halved, as one of two
+// numbers of 32 bits may pass them and t brings it back; below 1 such a difference has weight 0 in any case.
+struct Heat {
+    float half, rate;
+    __device__ __forceinline__ explicit Heat(float t) {
+        half = t >= 1.f ? 0.5f : 1.f;
+        // within float's range: a subnormal t must not make 0 rate a NaN
+        rate = fminf(kLog2e / (half * t), 3e38f);
+    }
+    // The bound takes -infinity (also at an infinite t) to 0; m is finite.
+    __device__ __forceinline__ float weight(float l, float m) const {
+        return __builtin_amdgcn_exp2f(fmaxf(fmaf(l, half, -half * m) * rate, -200.f));
+    }
+};
 
 // kVec logits from i on, -infinity where no token is allowed or the place is before `own`
 template <class T>
@@ -333,13 +339,13 @@ struct ProbRow {
         for (int i = 1; i < THREADS / 64; i++) top = fmaxf(top, part[i]);
     }
     // values become weights against `m`; their sum over all threads
-    __device__ __forceinline__ float weights(float m, float c) {
+    __device__ __forceinline__ float weights(float m, Heat heat) {
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < STEPS; j++)
 #pragma unroll
             for (int e = 0; e < kVec; e++) {
-                v[j][e] = weight_of(v[j][e], m, c);
+                v[j][e] = heat.weight(v[j][e], m);
                 sum += v[j][e];
             }
         __shared__ float part[THREADS / 64];
@@ -407,7 +413,7 @@ k_prob_rows(ProbArgs a) {
         return write_nan(mask, out, 0, a.vocab, THREADS);
     const bool greedy = t == 0.f;
     const uint32_t at = greedy && r.top > -infinity() ? r.first(r.top, 0, a.vocab) : 0xffffffffu;
-    const float sum = r.weights(r.top == -infinity() ? 0.f : r.top, rate_of(t));
+    const float sum = r.weights(r.top == -infinity() ? 0.f : r.top, Heat(t));
     const float scale = sum > 0.f ? 1.f / sum : 0.f;
     const uint32_t last = a.vocab - kVec;
 #pragma unroll
@@ -450,7 +456,7 @@ k_prob_parts(ProbArgs a) {
     else if (t == 0.f)
         p.first = r.top == -infinity() ? 0xffffffffu : r.first(r.top, begin, end);
     else
-        p.sum = r.weights(r.top == -infinity() ? 0.f : r.top, rate_of(t));
+        p.sum = r.weights(r.top == -infinity() ? 0.f : r.top, Heat(t));
     if (threadIdx.x == 0) static_cast<ProbPart *>(a.parts)[job] = p;
 }
 
@@ -467,7 +473,7 @@ k_prob_write(ProbArgs a) {
     const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
     float *out = a.out + row * a.vocab;
     const float t = a.temperatures ? a.temperatures[row] : a.temperature;
-    const float c = rate_of(t);
+    const Heat heat(t);
     float v[STEPS][kVec];
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {
@@ -488,7 +494,7 @@ k_prob_write(ProbArgs a) {
     for (uint32_t i = threadIdx.x; i < a.chunks; i += kChunkThreads) {
         const ProbPart p = parts[i];
         if (t == 0.f && p.top == top) first = min(first, p.first);
-        sum += t == 0.f ? p.sum : p.sum == 0.f ? 0.f : p.sum * weight_of(p.top, m, c);
+        sum += t == 0.f ? p.sum : p.sum == 0.f ? 0.f : p.sum * heat.weight(p.top, m);
     }
     sum = wave_sum(sum);
     first = ~wave_max(~first);
@@ -511,7 +517,7 @@ k_prob_write(ProbArgs a) {
         const uint32_t own = begin + (j * kChunkThreads + threadIdx.x) * kVec, i = min(own, last);
 #pragma unroll
         for (int e = 0; e < kVec; e++)
-            v[j][e] = t == 0.f ? (i + e == first ? 1.f : 0.f) : weight_of(v[j][e], m, c) * scale;
+            v[j][e] = t == 0.f ? (i + e == first ? 1.f : 0.f) : heat.weight(v[j][e], m) * scale;
         if (own < end) store_vec<kVec>(out + i, v[j]);
     }
 }
@@ -541,12 +547,13 @@ k_prob_short(ProbArgs a) {
         for (uint32_t i = 0; i < a.vocab; i++) out[i] = !mask || mask[i] ? not_a_number() : 0.f;
         return;
     }
-    const float c = rate_of(t), m = top == -infinity() ? 0.f : top;
+    const Heat heat(t);
+    const float m = top == -infinity() ? 0.f : top;
     for (int write = 0; write < 2; write++) {
         const float scale = sum > 0.f ? 1.f / sum : 0.f;
         for (uint32_t i = 0; i < a.vocab; i++) {
             const float l = !mask || mask[i] ? (float)logits[i] : -infinity();
-            const float w = t == 0.f ? (i == first ? 1.f : 0.f) : weight_of(l, m, c);
+            const float w = t == 0.f ? (i == first ? 1.f : 0.f) : heat.weight(l, m);
             if (write)
                 out[i] = w * scale;
             else

@@ -120,3 +120,18 @@ def test_logits_of_the_types_range(dev, dtype, rows, vocab):
         for m in (None, mask):
             p = ph.token_probabilities(x.to(dev), t.to(dev), None if m is None else m.to(dev))
             check_probs(p, f64(x), f64(t), None if m is None else m.numpy())
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 5), (4, 300), (4, 9000), (70, 20000), (4, 131072)])
+def test_subnormal_temperatures(dev, rows, vocab):
+    """Temperatures and differences of logits below 2^-126, down to where log2(e) / t passes 32 bits."""
+    import torch
+
+    x = torch.randint(-20, 1, (rows, vocab), generator=torch.Generator().manual_seed(vocab)) * 1e-39
+    x = x.to(torch.float32)
+    for heat in (4.9e-39, 7e-39, 1e-38):
+        t = torch.full((rows,), heat)
+        # t and c have 22 bits or more here: a relative error of 2^-21 in exponents of up to 4.1
+        p = f64(ph.token_probabilities(x.to(dev), t.to(dev)))
+        want = R.probabilities(f64(x), f64(t))
+        assert np.all(np.abs(p - want) <= (8.2 * 2.0 ** -21 + vocab / 64 * 2.0 ** -24) * want)
