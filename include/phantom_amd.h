@@ -481,6 +481,61 @@ int pfa_verify_drafts(const void *drafts, int token_bytes, const void *lengths, 
                       const float *noise, size_t noise_batch, void *tokens, int32_t *accepted, void *workspace,
                       size_t workspace_bytes, void *stream);
 
+/* Codes of 8-bit floating point (e4m3: 4 significant bits, largest 448, no infinity) of
+ * x [rows][width], with a scale for each 128 places of a row (block_rows 1) or for each 128
+ * rows and 128 places (block_rows 128).  A block's scale is the least power of two, 2^-126 or
+ * more, that takes its largest magnitude to 448 or less; code = x / scale to the nearest,
+ * ties to even.  A block of zeros has scale 0 and codes 0, one with a NaN or an infinity
+ * scale NaN and codes 0.  The scale of block (r, j) goes to scales[r scales_row + j
+ * scales_block]; pfa_fp8_matmul reads those of its left operand fastest where scales_row is 1. */
+int pfa_quantize_fp8(const void *x, size_t x_stride, int type, size_t rows, size_t width, size_t block_rows,
+                     uint8_t *codes, size_t codes_stride, float *scales, size_t scales_row, size_t scales_block,
+                     void *stream);
+
+/* y = x + residual (residual NULL: y = x), total = y rounded to `type` (written only
+ * with a residual); codes of y weight as pfa_quantize_fp8's with block_rows 1, the scales
+ * times 1 / sqrt(mean(y^2) + eps).  y, y weight and the sum of squares are formed in 32 bits: a
+ * block whose y weight is not finite there, and all blocks of a row whose sum is not, have
+ * scale NaN and codes 0.  Squares too small for 32 bits are not lost.  total must not
+ * overlap x or residual. */
+int pfa_rms_norm_fp8(const void *x, size_t x_stride, const void *residual, size_t residual_stride, const void *weight,
+                     int type, size_t rows, size_t width, double eps, void *total, size_t total_stride, uint8_t *codes,
+                     size_t codes_stride, float *scales, size_t scales_row, size_t scales_block, void *stream);
+
+/* Bytes of workspace that pfa_fp8_matmul needs for these sizes and type of outputs (0: none). */
+int pfa_fp8_workspace(size_t M, size_t N, size_t K, int type, size_t *bytes);
+
+/* out[m][n] = sum_j (sum_{k in block j} a[m][k] b[n][k]) a_scales(m, j) b_scales(n / 128, j) + bias[n]
+ * (bias NULL: none), blocks of 128 places, out of `type`.  a [M][K] and b [N][K] e4m3 codes;
+ * scale (r, j) at scales[r *_scales_row + j *_scales_block].  Sums are held in 32 bits.  For
+ * 16-bit outputs the matrix unit forms them: it adds eight neighbouring products aligned to the
+ * largest of them and cuts what is below 2^-13 of that one (towards 0).  For 32-bit
+ * outputs every product is added whole.  workspace: pfa_fp8_workspace bytes, otherwise as
+ * in pfa_int8_matmul. */
+int pfa_fp8_matmul(const uint8_t *a, size_t a_stride, const float *a_scales, size_t a_scales_row, size_t a_scales_block,
+                   const uint8_t *b, size_t b_stride, const float *b_scales, size_t b_scales_row, size_t b_scales_block,
+                   const float *bias, size_t M, size_t N, size_t K, void *out, int type, size_t out_stride,
+                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* Bytes of workspace that pfa_token_log_probs needs for these sizes (0: none). */
+int pfa_log_probs_workspace(size_t rows, size_t vocab, size_t *bytes);
+
+/* Log probabilities under softmax(logits / temperature) over the allowed places (logits,
+ * temperatures, mask as in pfa_token_probabilities): log_probs [rows][given] of tokens
+ * [rows][given], entropy [rows] in nats, and the `top` (64 at most) allowed places of the largest
+ * logits, larger ones first, the lowest place first among equals: top_tokens and
+ * top_log_probs [rows][top].  Tokens have token_bytes (4 or 8).  A token outside the vocabulary or
+ * not allowed has -infinity.  Where fewer than `top` places have a logit above -infinity,
+ * -1 and -infinity follow.  At temperature 0 the lowest place of the largest logit has
+ * 0, every other -infinity, the entropy is 0 and the alternatives are by their logits.  A row that
+ * allows nothing has -infinity and entropy 0.  Where pfa_token_probabilities says NaN, the row's
+ * numbers are NaN (those of tokens that are not allowed -infinity) and top_tokens -1.
+ * workspace: pfa_log_probs_workspace bytes, otherwise as in pfa_int8_matmul. */
+int pfa_token_log_probs(const void *logits, size_t stride, int type, size_t rows, size_t vocab, const void *tokens,
+                        int token_bytes, size_t given, size_t top, const float *temperatures, double temperature,
+                        const uint8_t *mask, size_t mask_stride, float *log_probs, float *entropy, float *top_log_probs,
+                        void *top_tokens, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,9 +3,10 @@
 A server that evaluates a model under encryption hands back the ciphertext of a
 hidden state; only the holder of the key can turn it into an answer.  These are
 the operators the holder runs on decrypted states: the norm, products with clear
-weights in 8 bits, probabilities, and the check of drafted tokens (an encrypted
-pass takes so long that several drafted tokens are checked per pass).  Callers use
-them through pyPhantom, which re-exports them.
+weights in 8 bits (integers with a scale a row, or floating point with a scale for
+each block of 128), probabilities and log probabilities, and the check of drafted
+tokens (an encrypted pass takes so long that several drafted tokens are checked per
+pass).  Callers use them through pyPhantom, which re-exports them.
 
 They take torch tensors on a GPU, launch on torch's current stream of the tensors'
 device, return new tensors (rms_norm_int8 without a residual returns x itself as the
@@ -21,7 +22,8 @@ import torch
 
 import pfa_native as _N
 
-__all__ = ["quantize_int8", "rms_norm_int8", "int8_matmul", "token_probabilities", "verify_drafts"]
+__all__ = ["quantize_int8", "rms_norm_int8", "int8_matmul", "quantize_fp8", "rms_norm_fp8", "fp8_matmul",
+           "token_probabilities", "token_log_probs", "verify_drafts"]
 
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PFA_F32, PFA_BF16, PFA_F16
 # the handle of the current stream of a device: torch.cuda.current_stream without the object
@@ -91,6 +93,33 @@ def _vector(t, n, dtype, name):
     return t
 
 
+def _temperature(logits, temperature):
+    """(a tensor with one for each row or None, the number for all of them)."""
+    if isinstance(temperature, torch.Tensor):
+        if temperature.dtype != torch.float32 or temperature.shape != logits.shape[:-1] or \
+                not temperature.is_contiguous():
+            _fail(f"temperature: expected a number or contiguous float32 {tuple(logits.shape[:-1])}")
+        return temperature, 0.0
+    one = float(temperature)
+    if not 0 <= one < float("inf"):
+        _fail("the temperature must be finite and 0 or more")
+    return None, one
+
+
+def _mask(logits, mask):
+    """(the mask as rows or as one row, distance of its rows; 0: one row for all)."""
+    if mask is None:
+        return None, 0
+    vocab = logits.shape[-1]
+    if mask.dtype != torch.bool or (mask.shape != logits.shape and mask.shape != (vocab,)):
+        _fail(f"mask: expected bool of {tuple(logits.shape)} or ({vocab},), got {tuple(mask.shape)} of {mask.dtype}")
+    if mask.dim() == 1 and vocab > 1 and mask.stride(0) != 1:
+        _fail("mask: the places of a row must be adjacent")
+    if mask.shape == logits.shape and logits.dim() > 1:
+        return _matrix(mask, "mask")
+    return mask, 0
+
+
 def _new(like, shape, dtype):
     """An empty contiguous tensor on like's device (the strided call is the cheapest of torch's)."""
     dims = len(shape)
@@ -103,20 +132,39 @@ def _new(like, shape, dtype):
     return torch.empty_strided(shape, strides, dtype=dtype, device=like.device)
 
 
-def _new_codes(like):
+def _new_codes(like, dtype=torch.int8):
     """(codes of like's shape, distance of their rows): rows start at whole cache lines, which
     int8_matmul reads fastest (777 x 5003 x 2050 at 2176 bytes a row 18.4 us, at 2064 20.3 us)."""
     shape = like.shape
     width = shape[-1]
     stride = (width + 127) & ~127 if width > 128 else (width + 15) & ~15
     if stride == width or not like.numel():
-        return _new(like, shape, torch.int8), width
+        return _new(like, shape, dtype), width
     strides, step = [1], stride
     for n in shape[-2::-1]:
         strides.append(step)
         step *= n
     # made with these strides at once: a view of whole rows would cost another 1.3 us
-    return torch.empty_strided(shape, strides[::-1], dtype=torch.int8, device=like.device), stride
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=like.device), stride
+
+
+def _new_scales(like, rows, blocks):
+    """Scales [..., blocks] of like [..., width]: those of one block stand together in memory, as fp8_matmul reads them
+    fastest."""
+    strides, step = [rows], 1
+    for n in like.shape[-2::-1]:
+        strides.append(step)
+        step *= n
+    return torch.empty_strided((*like.shape[:-1], blocks), strides[::-1], dtype=torch.float32, device=like.device)
+
+
+def _scales(t, rows, blocks, name):
+    """(t [..., blocks] as a two-dimensional view, distance of rows, distance of blocks)."""
+    if t.dtype != torch.float32 or t.shape[-1:] != (blocks,):
+        _fail(f"{name}: expected float32 [..., {blocks}], got {tuple(t.shape)} of {t.dtype}")
+    if t.dim() != 2:
+        t = t.reshape(rows, blocks)
+    return t, *t.stride()
 
 
 def _workspace(need, device):
@@ -219,6 +267,122 @@ def int8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
     return out
 
 
+def quantize_fp8(x, block_rows=1):
+    """Codes of 8-bit floating point (torch.float8_e4m3fn) of x [..., width], with a scale for
+    each block of 128: (codes [..., width], scales float32), x ~ codes * scales.
+
+    block_rows 1 (activations): a scale for each 128 places of a row, scales [..., ceil(width /
+    128)].  block_rows 128 (weights, x [rows, width]): one for each 128 rows and 128 places,
+    scales [ceil(rows / 128), ceil(width / 128)].
+
+    scale = the least power of two, 2^-126 or more, with max|block| <= 448 scale; code = x /
+    scale (which is exact) to the nearest, ties to even.  Blocks of zeros have scale 0;
+    blocks with a NaN or an infinity have scale NaN and codes 0.  Rows of more than 128 codes
+    start at multiples of 128 bytes, and the scales of one block of activations stand
+    together (stride() says where).
+    """
+    kind = _type_of(x, "x")
+    _same_device(x)
+    if block_rows not in (1, 128):
+        _fail(f"block_rows: expected 1 or 128, got {block_rows}")
+    if block_rows == 128 and x.dim() != 2:
+        _fail(f"x: blocks of 128 rows need two dimensions, got {tuple(x.shape)}")
+    rows, stride = _matrix(x, "x")
+    n, width = rows.shape
+    codes, codes_stride = _new_codes(x, torch.float8_e4m3fn)
+    blocks = (width + 127) // 128
+    if block_rows == 1:
+        scales, steps = _new_scales(x, n, blocks), (1, n)
+    else:
+        scales, steps = _new(x, ((n + 127) // 128, blocks), torch.float32), (blocks, 1)
+    if n and width:
+        _call("pfa_quantize_fp8", x, rows.data_ptr(), stride, kind, n, width, block_rows, codes.data_ptr(), codes_stride,
+              scales.data_ptr(), *steps)
+    return codes, scales
+
+
+def rms_norm_fp8(x, weight, eps=1e-6, residual=None):
+    """Root-mean-square norm of x + residual as codes of 8-bit floating point: (codes
+    torch.float8_e4m3fn [..., width], scales float32 [..., ceil(width / 128)], total).
+
+    With y = x + residual: total = y in x's type (x itself without a residual); the codes are
+    quantize_fp8's of y * weight, from the unrounded y, and the scales its scales times 1 /
+    sqrt(mean(y^2) + eps).  x [..., width]; residual like x; weight [width]; all of one
+    type.  y, y weight and the sum of squares are formed in 32 bits: a block where y
+    weight is not finite there, and all of a row where the sum is not, have scale NaN and
+    codes 0.
+    """
+    kind = _type_of(x, "x")
+    _same_device(x, weight, residual)
+    if not 0 <= eps < float("inf"):
+        _fail("eps must be finite and 0 or more")
+    rows, stride = _matrix(x, "x")
+    n, width = rows.shape
+    if width == 0:
+        _fail("x: the mean of an empty row")
+    _vector(weight, width, x.dtype, "weight")
+    total, more, more_stride, total_stride = x, None, 0, 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            _fail(f"residual: expected {tuple(x.shape)} of {x.dtype}, got {tuple(residual.shape)} of {residual.dtype}")
+        more, more_stride = _matrix(residual, "residual")
+        total, total_stride = _new(x, x.shape, x.dtype), width
+    codes, codes_stride = _new_codes(x, torch.float8_e4m3fn)
+    scales = _new_scales(x, n, (width + 127) // 128)
+    if n:
+        _call("pfa_rms_norm_fp8", x, rows.data_ptr(), stride, more.data_ptr() if more is not None else None,
+              more_stride, weight.data_ptr(), kind, n, width, float(eps), total.data_ptr() if total_stride else None,
+              total_stride, codes.data_ptr(), codes_stride, scales.data_ptr(), 1, n)
+    return codes, scales, total
+
+
+def fp8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
+    """out[..., n] = sum_j (sum_{k in block j} a[..., k] b[n, k]) a_scales[..., j] b_scales[n // 128, j]
+    + bias[n], blocks of 128 places.
+
+    a torch.float8_e4m3fn [..., K] with a_scales float32 [..., ceil(K / 128)] (one for each 128
+    places of a token), b torch.float8_e4m3fn [N, K] with b_scales float32 [ceil(N / 128), ceil(K /
+    128)] (one for each 128 output channels and 128 places), as quantize_fp8 gives them; any
+    numbers may be scales, in any order in memory.  bias float32 [N]; out of out_dtype
+    (float32, bfloat16 or float16).
+
+    Sums are held in 32 bits.  For bfloat16 and float16 outputs the matrix unit's 8-bit products
+    are used, which add eight neighbouring products aligned to the largest of them and cut
+    what is below 2^-13 of that one (towards 0): about 2^-16 of the result's size on normal
+    values.  For float32 outputs every product counts whole, at up to half the speed where
+    the product is not bound by reading b.  Rows of a and b that start at multiples of 128
+    bytes are read fastest, and a_scales whose values of one block stand together.
+    """
+    kind = _TYPE.get(out_dtype)
+    if kind is None:
+        _fail(f"out_dtype: expected float32, bfloat16 or float16, got {out_dtype}")
+    if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
+        _fail(f"expected torch.float8_e4m3fn codes, got {a.dtype} and {b.dtype}")
+    _same_device(a, a_scales, b, b_scales, bias)
+    if b.dim() != 2 or a.dim() < 1 or a.shape[-1] != b.shape[1]:
+        _fail(f"shapes {tuple(a.shape)} and {tuple(b.shape)} do not multiply")
+    rows, a_stride = _matrix(a, "a")
+    cols, b_stride = _matrix(b, "b")
+    m, k = rows.shape
+    n = cols.shape[0]
+    blocks = (k + 127) // 128
+    if a_scales.shape[:-1] != a.shape[:-1] or a_scales.dim() != a.dim():
+        _fail(f"a_scales: expected {(*a.shape[:-1], blocks)}, got {tuple(a_scales.shape)}")
+    if b_scales.dim() != 2 or b_scales.shape[0] != (n + 127) // 128:
+        _fail(f"b_scales: expected {((n + 127) // 128, blocks)}, got {tuple(b_scales.shape)}")
+    sa, *sa_steps = _scales(a_scales, m, blocks, "a_scales")
+    sb, *sb_steps = _scales(b_scales, b_scales.shape[0], blocks, "b_scales")
+    if bias is not None:
+        _vector(bias, n, torch.float32, "bias")
+    out = _new(a, (*a.shape[:-1], n), out_dtype)
+    if m and n:
+        held, space, size = _workspace(_N.fp8_workspace(m, n, k, kind), out.device)
+        _call("pfa_fp8_matmul", a, rows.data_ptr(), a_stride, sa.data_ptr(), *sa_steps, cols.data_ptr(), b_stride,
+              sb.data_ptr(), *sb_steps, bias.data_ptr() if bias is not None else None, m, n, k, out.data_ptr(), kind, n,
+              space, size)
+    return out
+
+
 def token_probabilities(logits, temperature=1.0, mask=None):
     """softmax(logits / temperature) over the allowed places: float32 [..., vocab].
 
@@ -231,27 +395,8 @@ def token_probabilities(logits, temperature=1.0, mask=None):
     kind = _type_of(logits, "logits")
     rows, stride = _matrix(logits, "logits")
     n, vocab = rows.shape
-    temperatures, one = None, 0.0
-    if isinstance(temperature, torch.Tensor):
-        if temperature.dtype != torch.float32 or temperature.shape != logits.shape[:-1] or \
-                not temperature.is_contiguous():
-            _fail(f"temperature: expected a number or contiguous float32 {tuple(logits.shape[:-1])}")
-        temperatures = temperature
-    else:
-        one = float(temperature)
-        if not 0 <= one < float("inf"):
-            _fail("the temperature must be finite and 0 or more")
-    allowed, mask_stride = None, 0
-    if mask is not None:
-        if mask.dtype != torch.bool or (mask.shape != logits.shape and mask.shape != (vocab,)):
-            _fail(f"mask: expected bool of {tuple(logits.shape)} or ({vocab},), got {tuple(mask.shape)} of "
-                  f"{mask.dtype}")
-        if mask.dim() == 1 and vocab > 1 and mask.stride(0) != 1:
-            _fail("mask: the places of a row must be adjacent")
-        if mask.shape == logits.shape and logits.dim() > 1:
-            allowed, mask_stride = _matrix(mask, "mask")
-        else:
-            allowed = mask
+    temperatures, one = _temperature(logits, temperature)
+    allowed, mask_stride = _mask(logits, mask)
     _same_device(logits, temperatures, mask)
     out = _new(logits, logits.shape, torch.float32)
     if out.numel():
@@ -260,6 +405,50 @@ def token_probabilities(logits, temperature=1.0, mask=None):
               temperatures.data_ptr() if temperatures is not None else None, one,
               allowed.data_ptr() if allowed is not None else None, mask_stride, out.data_ptr(), space, size)
     return out
+
+
+def token_log_probs(logits, tokens, top=0, temperature=1.0, mask=None):
+    """Log probabilities under softmax(logits / temperature) over the allowed places: (log_probs
+    float32 like tokens, entropy float32 [...], top_log_probs float32 [..., top], top_tokens
+    [..., top] of tokens' type).
+
+    logits [..., vocab]; tokens int32 or int64, [...] (one for each row) or [..., given];
+    temperature and mask as for token_probabilities; natural logarithms.  The alternatives are
+    the `top` (64 at most) allowed places of the largest logits, larger ones first, the lowest
+    place first among equals.  A token outside the vocabulary (padding) or not allowed has
+    -infinity; where fewer than `top` places are allowed (with a logit above -infinity), -1 and
+    -infinity follow.  At temperature 0 the lowest place of the largest logit has 0, all others
+    have -infinity, the entropy is 0.  A row that allows nothing has -infinity everywhere and
+    entropy 0; where token_probabilities has NaN, a row's numbers are NaN and its top_tokens -1.
+    """
+    kind = _type_of(logits, "logits")
+    rows, stride = _matrix(logits, "logits")
+    n, vocab = rows.shape
+    size = _WHOLE.get(tokens.dtype)
+    if size is None:
+        _fail(f"tokens: expected int32 or int64, got {tokens.dtype}")
+    lead = logits.shape[:-1]
+    if tokens.shape != lead and (tokens.dim() != logits.dim() or tokens.shape[:-1] != lead):
+        _fail(f"tokens: expected {tuple(lead)} or {(*lead, 'given')}, got {tuple(tokens.shape)}")
+    if not tokens.is_contiguous():
+        _fail("tokens: expected contiguous")
+    given = 1 if tokens.shape == lead else tokens.shape[-1]
+    if not isinstance(top, int) or not 0 <= top <= 64:
+        _fail(f"top: expected 0 to 64, got {top}")
+    temperatures, one = _temperature(logits, temperature)
+    allowed, mask_stride = _mask(logits, mask)
+    _same_device(logits, tokens, temperatures, mask)
+    log_probs = _new(logits, tokens.shape, torch.float32)
+    entropy = _new(logits, lead, torch.float32)
+    top_log_probs = _new(logits, (*lead, top), torch.float32)
+    top_tokens = _new(logits, (*lead, top), tokens.dtype)
+    if n:
+        held, space, need = _workspace(_N.log_probs_workspace(n, vocab), entropy.device)
+        _call("pfa_token_log_probs", logits, rows.data_ptr(), stride, kind, n, vocab, tokens.data_ptr(), size, given, top,
+              temperatures.data_ptr() if temperatures is not None else None, one,
+              allowed.data_ptr() if allowed is not None else None, mask_stride, log_probs.data_ptr(), entropy.data_ptr(),
+              top_log_probs.data_ptr(), top_tokens.data_ptr(), space, need)
+    return log_probs, entropy, top_log_probs, top_tokens
 
 
 def verify_drafts(draft_tokens, target_probs, uniforms, noise, draft_probs=None, lengths=None):

@@ -85,6 +85,15 @@ SIGNATURES = {
     "pfa_token_probabilities": (_i32, [_vp, _sz, _i32, _sz, _sz, _vp, C.c_double, _vp, _sz, _vp, _vp, _sz, _vp]),
     "pfa_verify_drafts": (_i32, [_vp, _i32, _vp, _i32, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _sz, _i32, _vp, _vp,
                                  _sz, _vp, _vp, _vp, _sz, _vp]),
+    "pfa_quantize_fp8": (_i32, [_vp, _sz, _i32, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp]),
+    "pfa_rms_norm_fp8": (_i32, [_vp, _sz, _vp, _sz, _vp, _i32, _sz, _sz, C.c_double, _vp, _sz, _vp, _sz, _vp, _sz, _sz,
+                                _vp]),
+    "pfa_fp8_workspace": (_i32, [_sz, _sz, _sz, _i32, C.POINTER(_sz)]),
+    "pfa_fp8_matmul": (_i32, [_vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _sz, _sz, _sz, _vp, _i32, _sz, _vp,
+                              _sz, _vp]),
+    "pfa_log_probs_workspace": (_i32, [_sz, _sz, C.POINTER(_sz)]),
+    "pfa_token_log_probs": (_i32, [_vp, _sz, _i32, _sz, _sz, _vp, _i32, _sz, _sz, _vp, C.c_double, _vp, _sz, _vp, _vp,
+                                   _vp, _vp, _vp, _sz, _vp]),
 }
 
 
@@ -515,3 +524,19 @@ class NativeContext:
             raise ValueError("expected an int64 device tensor")
         call("pfa_poly_from_signed", self._h, coeffs_i64.data_ptr(), ptr(out), L, start,
              stream or stream_of(out))
+
+
+@functools.lru_cache(maxsize=1024)
+def fp8_workspace(m: int, n: int, k: int, kind: int) -> int:
+    """Bytes of workspace of fp8_matmul for these sizes and outputs of this type (PFA_F32, ...)."""
+    size = C.c_size_t(0)
+    call("pfa_fp8_workspace", m, n, k, kind, C.byref(size))
+    return int(size.value)
+
+
+@functools.lru_cache(maxsize=1024)
+def log_probs_workspace(rows: int, vocab: int) -> int:
+    """Bytes of workspace of token_log_probs for rows x vocab."""
+    size = C.c_size_t(0)
+    call("pfa_log_probs_workspace", rows, vocab, C.byref(size))
+    return int(size.value)

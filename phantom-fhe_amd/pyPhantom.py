@@ -20,8 +20,9 @@ std::random_device).  Errors follow the reference's centred binomial
 distribution with 21 + 21 coin flips (sigma ~ 3.24, src/prng.cu:222-243).
 
 The clear end of an encrypted generation step (`quantize_int8`,
-`rms_norm_int8`, `int8_matmul`, `token_probabilities`, `verify_drafts`) works
-on plain torch tensors; clear_ops.py holds it.
+`rms_norm_int8`, `int8_matmul`, `quantize_fp8`, `rms_norm_fp8`, `fp8_matmul`,
+`token_probabilities`, `token_log_probs`, `verify_drafts`) works on plain torch
+tensors; clear_ops.py holds it.
 """
 from __future__ import annotations
 
@@ -36,7 +37,8 @@ import pfa_native as _N
 
 __version__ = "amd-1"
 
-_CLEAR_OPS = ("quantize_int8", "rms_norm_int8", "int8_matmul", "token_probabilities", "verify_drafts")
+_CLEAR_OPS = ("quantize_int8", "rms_norm_int8", "int8_matmul", "quantize_fp8", "rms_norm_fp8", "fp8_matmul",
+              "token_probabilities", "token_log_probs", "verify_drafts")
 
 
 def __getattr__(name):
