@@ -505,6 +505,10 @@ int pfa_rms_norm_fp8(const void *x, size_t x_stride, const void *residual, size_
 /* Bytes of workspace that pfa_fp8_matmul needs for these sizes and type of outputs (0: none). */
 int pfa_fp8_workspace(size_t M, size_t N, size_t K, int type, size_t *bytes);
 
+/* How pfa_fp8_matmul forms a product of these sizes and outputs: as pfa_matmul_plan.  It says which kernel a size
+ * runs; sums are formed in its order. */
+int pfa_fp8_plan(size_t M, size_t N, size_t K, int type, size_t *tile_rows, size_t *tile_cols, size_t *splits);
+
 /* out[m][n] = sum_j (sum_{k in block j} a[m][k] b[n][k]) a_scales(m, j) b_scales(n / 128, j) + bias[n]
  * (bias NULL: none), blocks of 128 places, out of `type`.  a [M][K] and b [N][K] e4m3 codes;
  * scale (r, j) at scales[r *_scales_row + j *_scales_block].  Sums are held in 32 bits.  For

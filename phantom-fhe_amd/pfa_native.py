@@ -89,6 +89,7 @@ SIGNATURES = {
     "pfa_rms_norm_fp8": (_i32, [_vp, _sz, _vp, _sz, _vp, _i32, _sz, _sz, C.c_double, _vp, _sz, _vp, _sz, _vp, _sz, _sz,
                                 _vp]),
     "pfa_fp8_workspace": (_i32, [_sz, _sz, _sz, _i32, C.POINTER(_sz)]),
+    "pfa_fp8_plan": (_i32, [_sz, _sz, _sz, _i32, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz)]),
     "pfa_fp8_matmul": (_i32, [_vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _sz, _sz, _sz, _vp, _i32, _sz, _vp,
                               _sz, _vp]),
     "pfa_log_probs_workspace": (_i32, [_sz, _sz, C.POINTER(_sz)]),
@@ -540,3 +541,10 @@ def log_probs_workspace(rows: int, vocab: int) -> int:
     size = C.c_size_t(0)
     call("pfa_log_probs_workspace", rows, vocab, C.byref(size))
     return int(size.value)
+
+
+def fp8_plan(m: int, n: int, k: int, kind: int) -> tuple[int, int, int]:
+    """(rows, columns, parts of K) of the tiles that form fp8_matmul's outputs of this type; rows 0: few rows, b streamed."""
+    out = [C.c_size_t(0) for _ in range(3)]
+    call("pfa_fp8_plan", m, n, k, kind, *(C.byref(v) for v in out))
+    return tuple(int(v.value) for v in out)
