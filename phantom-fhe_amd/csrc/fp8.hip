@@ -58,14 +58,18 @@ __device__ __forceinline__ uint2 codes_of(const float (&v)[kVec], const Step &s)
 // A thread's kVec places of a row of `width`, the first at `own`.  The row's last vector starts early, so no load
 // stands behind a branch and all of a thread's are in flight at once; what it reads before `own` (or all of it,
 // behind the row's end) is another thread's and becomes 0.  Rows of fewer than kVec places are read one by one.
+// EVEN: whole vectors only.  What is read behind the end is then the last vector again, of the row's last block, and
+// changes no largest: nothing is cleared.
+template <bool EVEN>
 struct Part {
     uint32_t own, at, width;
     __device__ __forceinline__ Part(uint32_t own, uint32_t width)
         : own(own), at(width >= kVec ? min(own, width - kVec) : 0u), width(width) {}
     __device__ __forceinline__ bool mine(int e) const { return at + e >= own && (width >= kVec || at + e < width); }
+    __device__ __forceinline__ bool inside() const { return own < width; }
     template <class T>
     __device__ __forceinline__ void load(const T *x, float (&v)[kVec]) const {
-        if (width >= kVec) {
+        if (EVEN || width >= kVec) {
             load_vec<kVec>(x + at, v);
         } else {
 #pragma unroll
@@ -73,13 +77,14 @@ struct Part {
         }
     }
     __device__ __forceinline__ void clear(float (&v)[kVec]) const {
+        if (EVEN) return;
 #pragma unroll
         for (int e = 0; e < kVec; e++) v[e] = mine(e) ? v[e] : 0.f;
     }
     // 2- and 4-byte values; where the vector starts early it holds the neighbour's own values too
     template <class T>
     __device__ __forceinline__ void store(T *x, const float (&v)[kVec]) const {
-        if (width >= kVec) {
+        if (EVEN || width >= kVec) {
             if (own < width) store_vec<kVec>(x + at, v);
         } else {
 #pragma unroll
@@ -88,9 +93,9 @@ struct Part {
         }
     }
     __device__ __forceinline__ void store_codes(uint8_t *codes, uint2 w) const {
-        if (own + kVec <= width) {
+        if (EVEN ? inside() : own + kVec <= width) {
             __builtin_memcpy(codes + own, &w, kVec);
-        } else {
+        } else if (!EVEN) {
 #pragma unroll
             for (int e = 0; e < kVec; e++)
                 if (mine(e)) codes[at + e] = (uint8_t)((e < 4 ? w.x : w.y) >> (e % 4 * 8));
@@ -116,7 +121,7 @@ struct BlockArgs {
 // blocks, all of a thread's loads in flight at once; the scales of its 16 rows stand together in memory.
 constexpr int kBlockRows = 16, kBlockSteps = 4;
 
-template <class T>
+template <class T, bool EVEN>
 __global__ void __launch_bounds__(256)
 k_fp8_rows(BlockArgs a) {
     const size_t job = row_of(), row = job / a.across * kBlockRows + threadIdx.x / kSpanLanes;
@@ -126,11 +131,11 @@ k_fp8_rows(BlockArgs a) {
     uint8_t *codes = a.codes + row * a.codes_stride;
     float v[kBlockSteps][kVec];
 #pragma unroll
-    for (int j = 0; j < kBlockSteps; j++) Part((first + j) * kSpan + lane * kVec, a.width).load(x, v[j]);
+    for (int j = 0; j < kBlockSteps; j++) Part<EVEN>((first + j) * kSpan + lane * kVec, a.width).load(x, v[j]);
 #pragma unroll
     for (int j = 0; j < kBlockSteps; j++) {
         const uint32_t block = first + j;
-        const Part p(block * kSpan + lane * kVec, a.width);
+        const Part<EVEN> p(block * kSpan + lane * kVec, a.width);
         p.clear(v[j]);
         const Step s(span_max(top_of(v[j])));
         p.store_codes(codes, codes_of(v[j], s));
@@ -140,14 +145,14 @@ k_fp8_rows(BlockArgs a) {
 }
 
 // A scale for each 128 rows and 128 places: a workgroup takes a block.
-template <class T>
+template <class T, bool EVEN>
 __global__ void __launch_bounds__(256)
 k_fp8_squares(BlockArgs a) {
     __shared__ uint32_t part[4];
     const size_t job = row_of(), down = job / a.across;
     if (down * kSpan >= a.rows) return;
     const uint32_t block = (uint32_t)(job % a.across);
-    const Part p(block * kSpan + threadIdx.x % kSpanLanes * kVec, a.width);
+    const Part<EVEN> p(block * kSpan + threadIdx.x % kSpanLanes * kVec, a.width);
     constexpr int kSteps = kSpan / (256 / kSpanLanes);
     float v[kSteps][kVec];
     uint32_t top = 0;
@@ -174,6 +179,17 @@ k_fp8_squares(BlockArgs a) {
     if (threadIdx.x == 0) a.scales[down * a.scales_row + block * a.scales_block] = __uint_as_float(s.scale);
 }
 
+template <class T, bool EVEN>
+void quantize_blocks(BlockArgs a, size_t block_rows, hipStream_t s) {
+    if (block_rows == 1) {
+        a.across = (a.across + kBlockSteps - 1) / kBlockSteps;
+        hipLaunchKernelGGL((k_fp8_rows<T, EVEN>), row_grid((a.rows + kBlockRows - 1) / kBlockRows * a.across), dim3(256), 0, s,
+                           a);
+    } else {
+        hipLaunchKernelGGL((k_fp8_squares<T, EVEN>), row_grid((a.rows + kSpan - 1) / kSpan * a.across), dim3(256), 0, s, a);
+    }
+}
+
 struct NormArgs {
     const void *x, *residual, *weight;
     void *total;
@@ -185,8 +201,8 @@ struct NormArgs {
 };
 
 // y = x + residual and v = y weight of a thread's places, the squares of y, total on the way
-template <class T>
-__device__ __forceinline__ void norm_values(const NormArgs &a, const T *x, const T *residual, T *total, const Part &p,
+template <class T, bool EVEN>
+__device__ __forceinline__ void norm_values(const NormArgs &a, const T *x, const T *residual, T *total, const Part<EVEN> &p,
                                             float &sum, float (&v)[kVec]) {
     float w[kVec];
     p.load(x, v);
@@ -199,19 +215,21 @@ __device__ __forceinline__ void norm_values(const NormArgs &a, const T *x, const
         if (total) p.store(total, v);
     }
     p.clear(v);
+    p.clear(w);
+    float squares = 0.f;
 #pragma unroll
     for (int e = 0; e < kVec; e++) {
-        sum = fmaf(v[e], v[e], sum);
+        squares = fmaf(v[e], v[e], squares);
         v[e] *= w[e];
     }
-    p.clear(v);  // 0 times an infinite weight
+    sum += p.inside() ? squares : 0.f;
 }
 
 // The norm's factor 1 / sqrt(mean + eps) is common to a row: codes and powers of two are those of the blocks of y
 // weight, and the factor goes into the scales.  So the row is read once and stays in registers, STEPS x kVec a thread,
 // while its squares are summed.  THREADS = 64: four rows a workgroup, one a wave, no barrier.  STEPS = 0:
 // rows too long for the registers are read twice.
-template <class T, int THREADS, int STEPS>
+template <class T, bool EVEN, int THREADS, int STEPS>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
 k_fp8_norm(NormArgs a) {
     constexpr bool kWave = THREADS == 64;
@@ -228,12 +246,12 @@ k_fp8_norm(NormArgs a) {
     uint32_t any = 0;  // of the row's magnitudes
     if (STEPS) {
 #pragma unroll
-        for (int j = 0; j < kHold; j++) norm_values(a, x, residual, total, Part((j * THREADS + t) * kVec, a.width), sum, v[j]);
+        for (int j = 0; j < kHold; j++) norm_values(a, x, residual, total, Part<EVEN>((j * THREADS + t) * kVec, a.width), sum, v[j]);
 #pragma unroll
         for (int j = 0; j < kHold; j++) any = max(any, top_of(v[j]));
     } else {
         for (uint32_t i = t * kVec; i < a.width; i += THREADS * kVec) {
-            norm_values(a, x, residual, total, Part(i, a.width), sum, v[0]);
+            norm_values(a, x, residual, total, Part<EVEN>(i, a.width), sum, v[0]);
             any = max(any, top_of(v[0]));
         }
     }
@@ -255,6 +273,19 @@ k_fp8_norm(NormArgs a) {
             any = max(any, part_any[w]);
         }
     }
+    // Codes first: they do not wait for the factor.
+    const bool lost = !(sum < __uint_as_float(kInfBits));
+    auto put_codes = [&](uint32_t i, const float (&u)[kVec]) {
+        Step s(span_max(top_of(u)));
+        s.bad |= lost;
+        if (i < a.width) Part<EVEN>(i, a.width).store_codes(codes, codes_of(u, s));
+        return s.bad ? kNan : s.scale;
+    };
+    uint32_t power[kHold];
+    if (STEPS) {
+#pragma unroll
+        for (int j = 0; j < kHold; j++) power[j] = put_codes((j * THREADS + t) * kVec, v[j]);
+    }
     // Squares below 2^-126 lose bits, below 2^-149 all of them.  Where they could matter, in a sum below
     // 2^-90 that eps does not outweigh, they are summed again.
     float lifted = 0.f;
@@ -273,34 +304,28 @@ k_fp8_norm(NormArgs a) {
     const double total_sum = few ? (double)lifted * 0x1p-200 : (double)sum;
     const double factor = few || a.eps > 0x1p100 ? rsqrt(total_sum / a.width + a.eps)
                                                  : (double)rsqrtf(sum / (float)a.width + (float)a.eps);
-    const bool lost = !(sum < __uint_as_float(kInfBits));
-    auto finish = [&](uint32_t i, const float (&u)[kVec]) {
-        Step s(span_max(top_of(u)));
-        s.bad |= lost;
-        Part(i, a.width).store_codes(codes, codes_of(u, s));
+    auto put_scale = [&](uint32_t i, uint32_t bits) {
         if (t % kSpanLanes == 0 && i < a.width)  // 0 stays 0 at eps = 0
-            scales[i / kSpan * a.scales_block] = s.bad     ? __uint_as_float(kNan)
-                                                 : s.scale ? (float)((double)__uint_as_float(s.scale) * factor)
-                                                           : 0.f;
+            scales[i / kSpan * a.scales_block] = bits ? (float)((double)__uint_as_float(bits) * factor) : 0.f;
     };
     if (STEPS) {
 #pragma unroll
-        for (int j = 0; j < kHold; j++) finish((j * THREADS + t) * kVec, v[j]);
+        for (int j = 0; j < kHold; j++) put_scale((j * THREADS + t) * kVec, power[j]);
     } else {
         float again = 0.f;
         // all lanes of a block go round together
         for (uint32_t i = t * kVec; i - t % kSpanLanes * kVec < a.width; i += THREADS * kVec) {
-            norm_values(a, x, residual, (T *)nullptr, Part(i, a.width), again, v[0]);
-            finish(i, v[0]);
+            norm_values(a, x, residual, (T *)nullptr, Part<EVEN>(i, a.width), again, v[0]);
+            put_scale(i, put_codes(i, v[0]));
         }
     }
 }
 
-template <class T>
+template <class T, bool EVEN>
 void norm_rows(const NormArgs &a, hipStream_t s) {
     const uint32_t vecs = (a.width + kVec - 1) / kVec;
 #define PFA_LAUNCH(threads, steps)                                                                                \
-    hipLaunchKernelGGL((k_fp8_norm<T, threads, steps>), row_grid(threads == 64 ? (a.rows + 3) / 4 : a.rows),      \
+    hipLaunchKernelGGL((k_fp8_norm<T, EVEN, threads, steps>), row_grid(threads == 64 ? (a.rows + 3) / 4 : a.rows),      \
                        dim3(threads < 256 ? 256 : threads), 0, s, a)
     if (vecs <= 64)
         PFA_LAUNCH(64, 1);
@@ -341,16 +366,13 @@ int pfa_quantize_fp8(const void *x, size_t x_stride, int type, size_t rows, size
         require((down == 1 || scales_row) && (across == 1 || scales_block), "pfa_quantize_fp8: scales overlap");
         aligned(x, size, "x");
         aligned(scales, 4, "scales");
-        BlockArgs a{x,        codes,        scales,     rows,         x_stride,
+        const BlockArgs a{x,        codes,        scales,     rows,         x_stride,
                     codes_stride, scales_row, scales_block, (uint32_t)width, (uint32_t)across};
-        if (block_rows == 1) a.across = (a.across + kBlockSteps - 1) / kBlockSteps;
         with_type(type, [&](auto t) {
-            using T = decltype(t);
-            if (block_rows == 1)
-                hipLaunchKernelGGL(k_fp8_rows<T>, row_grid((rows + kBlockRows - 1) / kBlockRows * a.across), dim3(256), 0,
-                                   as_stream(stream), a);
+            if (width % kVec)
+                quantize_blocks<decltype(t), false>(a, block_rows, as_stream(stream));
             else
-                hipLaunchKernelGGL(k_fp8_squares<T>, row_grid(down * a.across), dim3(256), 0, as_stream(stream), a);
+                quantize_blocks<decltype(t), true>(a, block_rows, as_stream(stream));
         });
         PFA_HIP(hipGetLastError());
     });
@@ -379,7 +401,12 @@ int pfa_rms_norm_fp8(const void *x, size_t x_stride, const void *residual, size_
         const NormArgs a{x,        residual,        weight,       total,        codes,      scales,       rows,
                          x_stride, residual_stride, total_stride, codes_stride, scales_row, scales_block, (uint32_t)width,
                          eps};
-        with_type(type, [&](auto t) { norm_rows<decltype(t)>(a, as_stream(stream)); });
+        with_type(type, [&](auto t) {
+            if (width % kVec)
+                norm_rows<decltype(t), false>(a, as_stream(stream));
+            else
+                norm_rows<decltype(t), true>(a, as_stream(stream));
+        });
         PFA_HIP(hipGetLastError());
     });
 }

@@ -14,7 +14,8 @@ pytestmark = pytest.mark.gpu
 
 U = R.U
 HALF = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}  # half a step, relative
-WIDTHS = [1, 2, 7, 8, 9, 63, 100, 127, 128, 129, 255, 256, 500, 1000, 1024, 2050, 4096, 5119, 8192, 16384, 20003, 40001]
+WIDTHS = [1, 2, 7, 8, 9, 63, 100, 127, 128, 129, 200, 255, 256, 500, 1000, 1024, 2050, 4096, 5119, 8192, 16384, 20003, 24576, 40001,
+          40960]
 
 
 def numbers(codes):
