@@ -520,11 +520,12 @@ struct Shape {
     uint32_t rows, cols;
     Cost narrow, wide;
 };
-enum { kSmall, kSquare, kBroad, kLarge, kHuge, kTall, kVast, kShapes };
+enum { kSmall, kSquare, kBroad, kLarge, kHigh, kHuge, kTall, kVast, kShapes };
 constexpr Shape shapes[kShapes] = {{32, 64, {.21f, .28f, .15f, .3f}, {.38f, .52f, .24f, .3f}},
                                    {64, 64, {.26f, .42f, .21f, .5f}, {.43f, .71f, .35f, .5f}},
                                    {64, 128, {.42f, .68f, .32f, 1.f}, {.65f, 1.1f, .55f, 1.f}},
                                    {128, 128, {.55f, 1.12f, .57f, 2.f}, {.94f, 1.87f, .96f, 3.f}},
+                                   {192, 128, {.73f, 1.48f, .73f, 3.5f}, {}},
                                    {128, 256, {.91f, 1.83f, .90f, 4.f}, {}},
                                    {256, 128, {.90f, 1.84f, .90f, 4.f}, {}},
                                    {256, 256, {1.6f, 3.3f, 1.66f, 6.5f}, {}}};
@@ -593,6 +594,7 @@ void matmul(const Fp8Args &g, const Plan &p, hipStream_t s) {
         case kLarge: return launch_tiles<T, 128, 128, 2, 4, 4>(g, s);
     }
     if constexpr (!std::is_same_v<T, float>) {
+        if (p.shape == kHigh) return launch_tiles<T, 192, 128, 4, 2, 3>(g, s);
         if (p.shape == kHuge) return launch_tiles<T, 128, 256, 2, 4, 3>(g, s);
         if (p.shape == kVast) return launch_tiles<T, 256, 256, 4, 2, 2>(g, s);
         return launch_tiles<T, 256, 128, 4, 2, 3>(g, s);
