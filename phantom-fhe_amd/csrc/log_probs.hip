@@ -7,7 +7,7 @@
 // are as many places' logits: their k-th largest has k places at or above it, so the k largest of the row are among
 // the places that reach it.  Those are collected (about k of them where the classes share them out evenly) and
 // ranked by comparing each with all.  Where they are too many to collect (long ties, logits in step with the
-// classes), the k-th largest of what was collected is the next threshold, until they fit.
+// classes), they are thrown into other classes, whose k-th largest is the next threshold.
 #include <algorithm>
 #include <cmath>
 
@@ -22,7 +22,7 @@ constexpr int kRowThreads = 1024;                      // of a long row where ro
 constexpr int kJoinThreads = 512;                      // that join a row's stretches
 constexpr int kUnroll = 4;                             // vectors of a thread on their way at once
 constexpr uint32_t kMostTop = 64;        // alternatives: at most half of the classes of places
-constexpr uint32_t kKept = 512;          // places that one collection holds
+constexpr uint32_t kKept = 512;          // places that one collection holds (9 bits number them)
 constexpr uint32_t kListed = 1024;       // groups of places that a collection looks at, all of them where more reach it
 constexpr uint32_t kRowGroups = 2048;    // groups of places a whole row
 constexpr uint32_t kChunkGroups = 16;    // groups of places a stretch
@@ -229,7 +229,8 @@ template <int THREADS, class R, class V, class F>
 __device__ __forceinline__ void largest(Shared<THREADS> &s, const R &row, uint32_t k, uint32_t floor, const float *tops,
                                         uint32_t groups, uint32_t vectors, V vector, F put) {
     uint64_t limit = max((uint64_t)floor << 32, (uint64_t)1);
-    for (;;) {
+    // f(key) for every place that reaches the limit
+    auto scan = [&](auto f) {
         __syncthreads();
         if (threadIdx.x == 0) s.count = s.listed = 0;
         __syncthreads();
@@ -250,18 +251,29 @@ __device__ __forceinline__ void largest(Shared<THREADS> &s, const R &row, uint32
 #pragma unroll
             for (int e = 0; e < kVec; e++) {
                 const uint64_t key = key_of(v[e], at + e);
-                if (key >= limit) {
-                    const uint32_t c = atomicAdd(&s.count, 1u);
-                    if (c < kKept) s.kept[c] = key;
-                }
+                if (key >= limit) f(key);
             }
         }
         __syncthreads();
+    };
+    for (uint32_t turn = 1;; turn += 2) {
+        scan([&](uint64_t key) {
+            const uint32_t n = atomicAdd(&s.count, 1u);
+            if (n < kKept) s.kept[n] = key;
+        });
         const uint32_t count = s.count;
         if (count <= kKept) return rank_kept(s, count, k, put);
+        // Too many: the largest of kKept classes that places are thrown into, others each time.  Their k-th largest
+        // leaves about k places, whatever the row looks like.
+        for (uint32_t i = threadIdx.x; i < kKept; i += THREADS) s.kept[i] = 0;
+        if (threadIdx.x == 0) s.limit = limit;
+        scan([&](uint64_t key) {
+            const uint32_t into = (uint32_t)key * (0x9e3779b1u * turn) >> 23;
+            atomicMax((unsigned long long *)&s.kept[into], (unsigned long long)key);
+        });
         rank_kept(s, kKept, k, [](uint32_t, uint64_t) {});
         __syncthreads();
-        limit = s.limit;
+        limit = max(limit, s.limit);  // 0 where fewer than k classes have a place
     }
 }
 
