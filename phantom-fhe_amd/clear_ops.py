@@ -29,7 +29,8 @@ _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PFA_F32, PFA_
 # the handle of the current stream of a device: torch.cuda.current_stream without the object
 # around it, which costs a call of a few microseconds more than its launch
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch.cuda.current_device
+# the current device: torch.cuda.current_device without its look at whether the GPU is in use yet, which a tensor on it says
+_current_device = torch._C._cuda_getDevice
 _WHOLE = {torch.int32: 4, torch.int64: 8}
 
 
@@ -158,13 +159,11 @@ def _new_scales(like, rows, blocks):
     return torch.empty_strided((*like.shape[:-1], blocks), strides[::-1], dtype=torch.float32, device=like.device)
 
 
-def _scales(t, rows, blocks, name):
-    """(t [..., blocks] as a two-dimensional view, distance of rows, distance of blocks)."""
-    if t.dtype != torch.float32 or t.shape[-1:] != (blocks,):
-        _fail(f"{name}: expected float32 [..., {blocks}], got {tuple(t.shape)} of {t.dtype}")
-    if t.dim() != 2:
-        t = t.reshape(rows, blocks)
-    return t, *t.stride()
+def _scales(t, shape, name):
+    """t [..., blocks], of `shape`, as a two-dimensional view; its strides say where its values are."""
+    if t.shape != shape or t.dtype != torch.float32:
+        _fail(f"{name}: expected float32 {tuple(shape)}, got {tuple(t.shape)} of {t.dtype}")
+    return t if len(shape) == 2 else t.reshape(shape[:-1].numel(), shape[-1])
 
 
 def _workspace(need, device):
@@ -359,26 +358,22 @@ def fp8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
     if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
         _fail(f"expected torch.float8_e4m3fn codes, got {a.dtype} and {b.dtype}")
     _same_device(a, a_scales, b, b_scales, bias)
-    if b.dim() != 2 or a.dim() < 1 or a.shape[-1] != b.shape[1]:
-        _fail(f"shapes {tuple(a.shape)} and {tuple(b.shape)} do not multiply")
+    shape = a.shape
+    if b.dim() != 2 or not shape or shape[-1] != b.shape[1]:
+        _fail(f"shapes {tuple(shape)} and {tuple(b.shape)} do not multiply")
     rows, a_stride = _matrix(a, "a")
     cols, b_stride = _matrix(b, "b")
-    m, k = rows.shape
-    n = cols.shape[0]
+    (m, k), n = rows.shape, b.shape[0]
     blocks = (k + 127) // 128
-    if a_scales.shape[:-1] != a.shape[:-1] or a_scales.dim() != a.dim():
-        _fail(f"a_scales: expected {(*a.shape[:-1], blocks)}, got {tuple(a_scales.shape)}")
-    if b_scales.dim() != 2 or b_scales.shape[0] != (n + 127) // 128:
-        _fail(f"b_scales: expected {((n + 127) // 128, blocks)}, got {tuple(b_scales.shape)}")
-    sa, *sa_steps = _scales(a_scales, m, blocks, "a_scales")
-    sb, *sb_steps = _scales(b_scales, b_scales.shape[0], blocks, "b_scales")
+    sa = _scales(a_scales, torch.Size((*shape[:-1], blocks)), "a_scales")
+    sb = _scales(b_scales, ((n + 127) // 128, blocks), "b_scales")
     if bias is not None:
         _vector(bias, n, torch.float32, "bias")
-    out = _new(a, (*a.shape[:-1], n), out_dtype)
+    out = _new(a, (m, n) if len(shape) == 2 else (*shape[:-1], n), out_dtype)
     if m and n:
         held, space, size = _workspace(_N.fp8_workspace(m, n, k, kind), out.device)
-        _call("pfa_fp8_matmul", a, rows.data_ptr(), a_stride, sa.data_ptr(), *sa_steps, cols.data_ptr(), b_stride,
-              sb.data_ptr(), *sb_steps, bias.data_ptr() if bias is not None else None, m, n, k, out.data_ptr(), kind, n,
+        _call("pfa_fp8_matmul", a, rows.data_ptr(), a_stride, sa.data_ptr(), *sa.stride(), cols.data_ptr(), b_stride,
+              sb.data_ptr(), *sb.stride(), bias.data_ptr() if bias is not None else None, m, n, k, out.data_ptr(), kind, n,
               space, size)
     return out
 
