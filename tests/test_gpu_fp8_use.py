@@ -223,3 +223,22 @@ def test_outputs_past_32_bits(dev):
     out = ph.fp8_matmul(a, sa, b, sb, None, torch.bfloat16)
     assert out[0, 0] == 1 and out[-1, -1] == k and out[-1, 0] == 1 and out[0, -1] == 1
     assert int((out != 0).sum()) == 4
+
+
+def test_example(dev):
+    """examples/encrypted_decoding.py with the vocabulary in 8-bit floats runs, and says the tokens it kept."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "encrypted_decoding.py")
+    spec = importlib.util.spec_from_file_location("encrypted_decoding", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    lines = []
+    text, worst = module.run(rounds=2, say=lines.append, codes="e4m3")
+    assert 2 <= len(text) <= 10 and all(0 <= t < 1000 for t in text) and len(lines) == 3
+    # A code is off by 2^-4 of itself at most: a logit of deviation 1 by less than 2^-4 (both factors, independent, uniform
+    # within their steps), probabilities by 2^-4 / 0.8 = 0.08 in the mean at most
+    assert worst < 0.1
+    with pytest.raises(ValueError):
+        module.run(codes="fp4")
