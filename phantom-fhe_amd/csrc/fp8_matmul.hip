@@ -182,7 +182,7 @@ k_fp8_tiles(Fp8Args g) {
     constexpr int kRows = BM + BN, kCodes = kRows * kBlock;
     constexpr int kStage = kCodes + WAVES * 256, kScaleB = (BM + 63) / 64 * 64;  // a's scales, then b's
     constexpr int kLoads = kRows / 8 / WAVES;  // a wave's load is 8 rows, 1 KiB
-        static_assert(kRows % (8 * WAVES) == 0 && BM % 8 == 0, "whole loads");
+    static_assert(kRows % (8 * WAVES) == 0 && BM % 8 == 0, "whole loads");
     static_assert(kScaleB < WAVES * 64, "a load of scales each wave");
     static_assert(BN % 64 == 0 && 128 % (BN / WN) == 0 && 256 % BN == 0, "a wave's columns share their scales");
     // the ring, and in its place behind the products a line of outputs a wave
@@ -191,7 +191,7 @@ k_fp8_tiles(Fp8Args g) {
     static_assert(kLds <= 160 * 1024, "a CU's LDS");
     __shared__ __align__(1024) int8_t held[kLds];
     uint32_t start = 0;
-    asm("" : "+s"(start));  // as in int8_matmul's tiles
+    asm("" : "+s"(start));  // where the ring begins is not told to the compiler: it moves sums between registers otherwise
     int8_t *ring = held + start;
     // a wave's number is said to be uniform: addresses of loads and places in the ring are then scalar
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -661,7 +661,8 @@ int pfa_fp8_matmul(const uint8_t *a, size_t a_stride, const float *a_scales, siz
         if ((M > 1 && (a_stride > far || a_scales_row > far / 8)) || (N > 1 && b_stride > far) ||
             (N > kBlock && b_scales_row > far))
             p = {true, 0, 1};
-        require(!p.few || M <= 65535 * 16, "pfa_fp8_matmul: rows this far apart: at most 1048560 of a");
+        require(!p.few || (M <= 65535 * 16 && N < (size_t)1 << 27),
+                "pfa_fp8_matmul: rows this far apart: at most 1048560 of a and 2^27 - 1 of b");
         const size_t need = parts_bytes(M, N, p);
         require(workspace_bytes >= need, "pfa_fp8_matmul: the workspace needs " + std::to_string(need) + " bytes");
         require(((uintptr_t)workspace & 15) == 0, "pfa_fp8_matmul: the workspace is not aligned to 16 bytes");
