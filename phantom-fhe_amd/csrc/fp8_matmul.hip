@@ -512,7 +512,7 @@ k_fp8_join(Fp8Args g) {
 
 // The shapes of k_fp8_tiles and what they cost a CU, in us (measured, gfx950, over K from 512 to 8192): a block of K
 // `alone` with one tile a CU, `pair` with two, `each` for every one of more, and `end` for a tile's start and outputs;
-// of 16-bit outputs, then of 32-bit ones, which the largest shapes are not built for.
+// of 16-bit outputs, then of 32-bit ones, which the largest shape is not built for.
 struct Cost {
     float alone, pair, each, end;
 };
@@ -525,9 +525,9 @@ constexpr Shape shapes[kShapes] = {{32, 64, {.21f, .28f, .15f, .3f}, {.38f, .52f
                                    {64, 64, {.26f, .42f, .21f, .5f}, {.43f, .71f, .35f, .5f}},
                                    {64, 128, {.42f, .68f, .32f, 1.f}, {.65f, 1.1f, .55f, 1.f}},
                                    {128, 128, {.55f, 1.12f, .57f, 2.f}, {.94f, 1.87f, .96f, 3.f}},
-                                   {192, 128, {.73f, 1.48f, .73f, 3.5f}, {}},
-                                   {128, 256, {.91f, 1.83f, .90f, 4.f}, {}},
-                                   {256, 128, {.90f, 1.84f, .90f, 4.f}, {}},
+                                   {192, 128, {.73f, 1.48f, .73f, 3.5f}, {1.27f, 2.55f, 1.35f, 3.5f}},
+                                   {128, 256, {.91f, 1.83f, .90f, 4.f}, {1.53f, 3.4f, 1.66f, 5.f}},
+                                   {256, 128, {.90f, 1.84f, .90f, 4.f}, {1.53f, 3.4f, 1.67f, 5.f}},
                                    {256, 256, {1.6f, 3.3f, 1.66f, 6.5f}, {}}};
 
 // How a product is formed: `few` by k_fp8_few, else by tiles of `shape`, K in `splits` parts.
@@ -549,9 +549,8 @@ Plan plan_matmul(size_t M, size_t N, size_t K, int type) {
     float least = INFINITY;
     for (int i = 0; i < kShapes; i++) {
         const Shape &s = shapes[i];
-        if (s.rows > 32 && M <= s.rows / 2) continue;          // half a tile or more of nothing
-        if (type == PFA_F32 && i > kLarge) continue;
-        if (i == kVast && K % kBlock) continue;                // takes whole blocks only
+        if (s.rows > 32 && M <= s.rows / 2) continue;                 // half a tile or more of nothing
+        if (i == kVast && (type == PFA_F32 || K % kBlock)) continue;  // takes whole blocks only
         const Cost &c = type == PFA_F32 ? s.wide : s.narrow;
         const size_t down = (M + s.rows - 1) / s.rows, tiles = down * ((N + s.cols - 1) / s.cols);
         const float reading = ((float)N * K * (1 + .15f * (down - 1)) + (float)M * K) / memory;
@@ -592,13 +591,12 @@ void matmul(const Fp8Args &g, const Plan &p, hipStream_t s) {
         case kSquare: return launch_tiles<T, 64, 64, 2, 2, 4>(g, s);
         case kBroad: return launch_tiles<T, 64, 128, 2, 2, 3>(g, s);
         case kLarge: return launch_tiles<T, 128, 128, 2, 4, 4>(g, s);
+        case kHigh: return launch_tiles<T, 192, 128, 4, 2, 3>(g, s);
+        case kHuge: return launch_tiles<T, 128, 256, 2, 4, 3>(g, s);
+        case kTall: return launch_tiles<T, 256, 128, 4, 2, 3>(g, s);
     }
-    if constexpr (!std::is_same_v<T, float>) {
-        if (p.shape == kHigh) return launch_tiles<T, 192, 128, 4, 2, 3>(g, s);
-        if (p.shape == kHuge) return launch_tiles<T, 128, 256, 2, 4, 3>(g, s);
+    if constexpr (!std::is_same_v<T, float>)
         if (p.shape == kVast) return launch_tiles<T, 256, 256, 4, 2, 2>(g, s);
-        return launch_tiles<T, 256, 128, 4, 2, 3>(g, s);
-    }
 }
 
 size_t parts_bytes(size_t M, size_t N, const Plan &p) {

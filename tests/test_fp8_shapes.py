@@ -22,6 +22,8 @@ def test_products_reach_every_tile(kind, sizes, tiles):
         whole = {k // 128 for _, _, k in mine}
         if t == (256, 256):  # takes whole blocks of K only
             assert all(k % 128 == 0 for _, _, k in mine) and {1, 2, 3} <= whole and max(whole) >= 4
+        elif kind == F32 and t[0] * t[1] > 128 * 128:  # for a block and more
+            assert {1, 2, 3} <= whole and max(whole) >= 4 and {k % 128 == 0 for _, _, k in mine} == {True, False}
         elif t == (192, 128):  # for three blocks and more
             assert 3 in whole and max(whole) >= 4 and {k % 128 == 0 for _, _, k in mine} == {True, False}
         elif (kind, t) != (F32, (128, 128)):  # that one is for long sums only
@@ -56,8 +58,8 @@ def test_nothing_is_spilled(kernels):
 
 
 @pytest.mark.parametrize("shape,groups,types", [("32, 64, 2, 2, 6", 2, 3), ("64, 64, 2, 2, 4", 2, 3), ("64, 128, 2, 2, 3", 2, 3),
-                                                ("128, 128, 2, 4, 4", 1, 3), ("192, 128, 4, 2, 3", 1, 2), ("128, 256, 2, 4, 3", 1, 2),
-                                                ("256, 128, 4, 2, 3", 1, 2), ("256, 256, 4, 2, 2", 1, 2)])
+                                                ("128, 128, 2, 4, 4", 1, 3), ("192, 128, 4, 2, 3", 1, 3), ("128, 256, 2, 4, 3", 1, 3),
+                                                ("256, 128, 4, 2, 3", 1, 3), ("256, 256, 4, 2, 2", 1, 2)])
 def test_tiles_fit(kernels, shape, groups, types):
     """As many workgroups as the costs of the shapes were measured with: 160 KiB of LDS a CU, 512 registers a lane of a
     SIMD.  The ring is part of the kernel."""
