@@ -119,6 +119,8 @@ struct BlockArgs {
 
 // A scale for each 128 places of a row.  16 lanes take a block of a row, a workgroup 16 rows and 4
 // blocks, all of a thread's loads in flight at once; the scales of its 16 rows stand together in memory.
+// Bound by memory: 4096 x 8192 bf16 17.4 us (5.8 TB/s), float32 28.4 (5.9 TB/s); rows that begin anywhere, 777 x 5119
+// fp16, 6.1 us.
 constexpr int kBlockRows = 16, kBlockSteps = 4;
 
 template <class T, bool EVEN>
@@ -144,7 +146,8 @@ k_fp8_rows(BlockArgs a) {
     }
 }
 
-// A scale for each 128 rows and 128 places: a workgroup takes a block.
+// A scale for each 128 rows and 128 places: a workgroup takes a block, 8 vectors a thread in flight at once, so that
+// the block is read once.  Bound by memory: 16384 x 4096 bf16 35 us (5.8 TB/s), float32 60 us (5.6 TB/s).
 template <class T, bool EVEN>
 __global__ void __launch_bounds__(256)
 k_fp8_squares(BlockArgs a) {
@@ -228,7 +231,8 @@ __device__ __forceinline__ void norm_values(const NormArgs &a, const T *x, const
 // The norm's factor 1 / sqrt(mean + eps) is common to a row: codes and powers of two are those of the blocks of y
 // weight, and the factor goes into the scales.  So the row is read once and stays in registers, STEPS x kVec a thread,
 // while its squares are summed.  THREADS = 64: four rows a workgroup, one a wave, no barrier.  STEPS = 0:
-// rows too long for the registers are read twice.
+// rows too long for the registers are read twice.  Bound by memory: 4096 x 8192 bf16 with residual 44-47 us (5.0-5.4
+// TB/s), float32 84 us (5.2 TB/s); one row of 4096 3.3 us.
 template <class T, bool EVEN, int THREADS, int STEPS>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
 k_fp8_norm(NormArgs a) {
