@@ -9,8 +9,8 @@ tokens (an encrypted pass takes so long that several drafted tokens are checked 
 pass).  Callers use them through pyPhantom, which re-exports them.
 
 They take torch tensors on a GPU, launch on torch's current stream of the tensors'
-device, return new tensors (rms_norm_int8 without a residual returns x itself as the
-total) and never wait for the GPU.  Rows may be strided, the elements of a row are
+device, return new tensors (rms_norm_int8 and rms_norm_fp8 without a residual return x
+itself as the total) and never wait for the GPU.  Rows may be strided, the elements of a row are
 adjacent.  Wrong arguments raise ValueError, as everywhere in pyPhantom.  They are for
 inference: what they return carries no gradient, whatever its inputs require, and
 they take real tensors only, not those of torch's tracing or vmap.  There is no CPU
@@ -282,7 +282,7 @@ def quantize_fp8(x, block_rows=1):
     """
     kind = _type_of(x, "x")
     _same_device(x)
-    if block_rows not in (1, 128):
+    if not isinstance(block_rows, int) or block_rows not in (1, 128):
         _fail(f"block_rows: expected 1 or 128, got {block_rows}")
     if block_rows == 128 and x.dim() != 2:
         _fail(f"x: blocks of 128 rows need two dimensions, got {tuple(x.shape)}")
@@ -342,8 +342,8 @@ def fp8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
     a torch.float8_e4m3fn [..., K] with a_scales float32 [..., ceil(K / 128)] (one for each 128
     places of a token), b torch.float8_e4m3fn [N, K] with b_scales float32 [ceil(N / 128), ceil(K /
     128)] (one for each 128 output channels and 128 places), as quantize_fp8 gives them; any
-    numbers may be scales, in any order in memory.  bias float32 [N]; out of out_dtype
-    (float32, bfloat16 or float16).
+    numbers may be scales, in any order in memory; the two of a block are multiplied first, in 32
+    bits.  bias float32 [N]; out of out_dtype (float32, bfloat16 or float16).
 
     Sums are held in 32 bits.  For bfloat16 and float16 outputs the matrix unit's 8-bit products
     are used, which add eight neighbouring products aligned to the largest of them and cut

@@ -24,6 +24,7 @@ F8, F32, BF16, I64, I32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, to
     (lambda: ph.quantize_fp8(fake(20).as_strided((4, 5), (3, 1))), "overlap"),
     (lambda: ph.quantize_fp8(fake()), "dimension"),
     (lambda: ph.quantize_fp8(fake(2, 3), 64), "block_rows"),
+    (lambda: ph.quantize_fp8(fake(2, 3), 1.0), "block_rows"),
     (lambda: ph.quantize_fp8(fake(2, 3, 4), 128), "two dimensions"),
     (lambda: ph.quantize_fp8(fake(4), 128), "two dimensions"),
     (lambda: ph.rms_norm_fp8(torch.zeros(2, 3), torch.zeros(3)), "GPU"),
