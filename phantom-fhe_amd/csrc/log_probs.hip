@@ -18,7 +18,7 @@ namespace pfa {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;  // of a row, and of a stretch of one
-constexpr int kRowThreads = 1024;                      // of a long row where rows are few
+constexpr int kRowThreads = 512;                       // of a long row where rows are few
 constexpr int kJoinThreads = 512;                      // that join a row's stretches
 constexpr int kUnroll = 4;                             // vectors of a thread on their way at once
 constexpr uint32_t kMostTop = 64;        // alternatives: at most half of the classes of places
@@ -521,13 +521,14 @@ struct LogCut {
     int threads;
 };
 
-// Measured, bf16, us, rows of 256 threads / of 1024 / cut (two launches): 1 row of 16384 8.1 / 10.0 / 12.9, of 32768 10.4 /
-// 9.7 / 13.0, of 65536 15.8 / 12.2 / 13.0, of 131072 24 / 16.2 / 13.0; 128 of 65536 17.2 / 14.2 / 18.5, of 131072 26 / 19
-// / 21; 320 of 131072 30 / 30 / 37.  Stretches have one vector a thread, and four where those would be more than eight
-// workgroups a CU.
+// Measured, bf16, us, rows of 256 threads / of 512 / cut (two launches): 16 rows of 8192 7.5 / 8.5, of 16384 8.5 / 8.3, of 32768
+// 10.3 / 9.7, of 65536 14.0 / 12.3 / 13, of 131072 21 / 18 / 13; 128 of 65536 16.5 / 13.6 / 18.5, of 131072 24.5 / 19.1 / 21;
+// 256 of 32768 12.5 / 11.3, of 131072 25 / 20; 320 of 32768 13.8 / 14.2, of 131072 float32 39 / 45.  1024 threads are 512's
+// equal at best (16 of 131072) and up to 2.5 us slower to begin and end.  Stretches have one vector a thread, and four
+// where those would be more than eight workgroups a CU.
 LogCut cut_log_probs(size_t rows, uint32_t vocab) {
     if (vocab <= 65536 || rows > vocab / 4096)
-        return {vocab, 1, vocab > 20000 && rows < 256 ? kRowThreads : kThreads};
+        return {vocab, 1, vocab >= 16384 && rows <= 256 ? kRowThreads : kThreads};
     const uint64_t least = kThreads * kVec, most = kMostGroups / kChunkGroups;  // places, stretches
     uint64_t chunk = rows * vocab <= 2048 * least && vocab <= least * most ? least : kUnroll * least;
     chunk *= (vocab + chunk * most - 1) / (chunk * most);

@@ -186,7 +186,7 @@ def test_crowded_rows(dev):
         rising = torch.where(few, i.float(), -1e6)
         rows = torch.stack([rising, torch.where(few, -i.float(), -1e7), torch.where(few, 1.0, 0.0)])
         tokens = torch.zeros(3, dtype=torch.int64, device=dev)
-        for more in (1, 400 if vocab == 131072 else 1):
+        for more in (1, 20, 400) if vocab == 131072 else (1,):  # cut rows, long and ordinary workgroups
             _, _, tops, places = ph.token_log_probs(rows.repeat(more, 1), tokens.repeat(more), 64)
             order = torch.sort(rows, dim=-1, descending=True, stable=True).indices[:, :64]
             assert torch.equal(places, order.repeat(more, 1)) and not torch.isnan(tops).any()
