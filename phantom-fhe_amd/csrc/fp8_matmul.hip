@@ -552,10 +552,13 @@ struct Plan {
 // The plan of least estimated time: that of the products and the tiles' ends, or of reading b, a little more for every
 // row of tiles that reads it again.  Few rows and few columns go to k_fp8_few (kernels, few / 32 x 64 tiles: 1 x 4096 x
 // 4096 7.8 / 9.6 us, float32 9.1 / 10.4; 16 x 8192 x 4096 12.4 / 11.3, float32 15.1 / 15.7; 16 x 16384 x 4096 20.6 /
-// 14.4).  K is split where tiles are too few for the card and the sums are long enough to pay for the second launch and
-// the partial sums (128 x 4096 x 16384: 59.8 us whole, 26.4 in 4).
+// 14.4), and what is at most a workgroup of it a CU, unless the sums are long (19 x 1414 x 1024 4.3 / 5.2, 120 x 405 x 3359
+// 8.9 / 11.9, 46 x 128 x 13056 15.1 / 10.7 with K split; 42 x 2595 x 1280, 489 workgroups, 7.1 / 5.6).  K is split
+// where tiles are too few for the card and the sums are long enough to pay for the second launch and the partial
+// sums (128 x 4096 x 16384: 59.8 us whole, 26.4 in 4).
 Plan plan_matmul(size_t M, size_t N, size_t K, int type) {
     if (M <= 16 && N <= 8192) return {true, 0, 1};
+    if ((M + 15) / 16 * ((N + 15) / 16) <= 256 && K <= 8192) return {true, 0, 1};
     const float blocks = (float)((K + kBlock - 1) / kBlock), memory = 5e6f;  // bytes a us
     Plan best{false, 0, 1};
     float least = INFINITY;

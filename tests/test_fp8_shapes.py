@@ -5,7 +5,7 @@ import re
 import pytest
 
 import pfa_native as P
-from fp8_shapes import NARROW, NARROW_TILES, WIDE, WIDE_TILES
+from fp8_shapes import FEW, NARROW, NARROW_TILES, WIDE, WIDE_TILES
 from test_clear_kernel_code import named
 from test_kernel_code import kernels  # noqa: F401
 
@@ -38,6 +38,7 @@ def test_products_reach_every_tile(kind, sizes, tiles):
 def test_plan():
     for kind in (F32, BF16, F16):
         assert P.fp8_plan(1, 4096, 4096, kind) == (0, 16, 1) and P.fp8_plan(16, 8192, 100, kind) == (0, 16, 1)
+        assert {P.fp8_plan(*size, kind) for size in FEW} == {(0, 16, 1)}
         assert P.fp8_plan(17, 4096, 4096, kind)[0] > 0 and P.fp8_plan(1, 8193, 4096, kind)[0] > 0
     assert P.fp8_plan(333, 777, 999, BF16) == P.fp8_plan(333, 777, 999, F16)
     for m, n, k in WIDE + NARROW:

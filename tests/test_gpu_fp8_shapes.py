@@ -3,7 +3,7 @@ import pytest
 
 import fp8_reference as R
 import pyPhantom as ph
-from fp8_shapes import NARROW, WIDE
+from fp8_shapes import FEW, NARROW, WIDE
 from test_gpu_clear_ops import dtype_of
 from test_gpu_fp8_ops import HALF, operands
 
@@ -39,7 +39,7 @@ def check_large(out, a, sa, b, sb, bias, dtype):
     assert bool((far <= room).all()), (float((far / room).max()), torch.nonzero(far > room)[:4].tolist())
 
 
-@pytest.mark.parametrize("m,n,k", WIDE)
+@pytest.mark.parametrize("m,n,k", WIDE + FEW)
 def test_wide(dev, m, n, k):
     import torch
 
@@ -49,7 +49,7 @@ def test_wide(dev, m, n, k):
         check_large(ph.fp8_matmul(*args, bias, torch.float32), *args, bias, "float32")
 
 
-@pytest.mark.parametrize("m,n,k", NARROW)
+@pytest.mark.parametrize("m,n,k", NARROW + FEW)
 def test_narrow(dev, m, n, k):
     import torch
 
