@@ -141,6 +141,8 @@ def _new_codes(like, dtype=torch.int8):
     stride = (width + 127) & ~127 if width > 128 else (width + 15) & ~15
     if stride == width or not like.numel():
         return _new(like, shape, dtype), width
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (stride, 1), dtype=dtype, device=like.device), stride
     strides, step = [1], stride
     for n in shape[-2::-1]:
         strides.append(step)
@@ -152,6 +154,8 @@ def _new_codes(like, dtype=torch.int8):
 def _new_scales(like, rows, blocks):
     """Scales [..., blocks] of like [..., width]: those of one block stand together in memory, as fp8_matmul reads them
     fastest."""
+    if like.dim() == 2:
+        return torch.empty_strided((rows, blocks), (1, rows), dtype=torch.float32, device=like.device)
     strides, step = [rows], 1
     for n in like.shape[-2::-1]:
         strides.append(step)
@@ -414,7 +418,8 @@ def token_log_probs(logits, tokens, top=0, temperature=1.0, mask=None):
     -infinity; where fewer than `top` places are allowed (with a logit above -infinity), -1 and
     -infinity follow.  At temperature 0 the lowest place of the largest logit has 0, all others
     have -infinity, the entropy is 0.  A row that allows nothing has -infinity everywhere and
-    entropy 0; where token_probabilities has NaN, a row's numbers are NaN and its top_tokens -1.
+    entropy 0; where token_probabilities has NaN, a row's numbers are NaN (those of tokens that
+    are not allowed -infinity) and its top_tokens -1.
     """
     kind = _type_of(logits, "logits")
     rows, stride = _matrix(logits, "logits")
@@ -422,21 +427,23 @@ def token_log_probs(logits, tokens, top=0, temperature=1.0, mask=None):
     size = _WHOLE.get(tokens.dtype)
     if size is None:
         _fail(f"tokens: expected int32 or int64, got {tokens.dtype}")
-    lead = logits.shape[:-1]
-    if tokens.shape != lead and (tokens.dim() != logits.dim() or tokens.shape[:-1] != lead):
-        _fail(f"tokens: expected {tuple(lead)} or {(*lead, 'given')}, got {tuple(tokens.shape)}")
+    lead, shape, given = logits.shape[:-1], tokens.shape, 1
+    if shape != lead:
+        if len(shape) != len(lead) + 1 or shape[:-1] != lead:
+            _fail(f"tokens: expected {tuple(lead)} or {(*lead, 'given')}, got {tuple(shape)}")
+        given = shape[-1]
     if not tokens.is_contiguous():
         _fail("tokens: expected contiguous")
-    given = 1 if tokens.shape == lead else tokens.shape[-1]
     if not isinstance(top, int) or not 0 <= top <= 64:
         _fail(f"top: expected 0 to 64, got {top}")
     temperatures, one = _temperature(logits, temperature)
     allowed, mask_stride = _mask(logits, mask)
     _same_device(logits, tokens, temperatures, mask)
-    log_probs = _new(logits, tokens.shape, torch.float32)
+    log_probs = _new(logits, shape, torch.float32)
     entropy = _new(logits, lead, torch.float32)
-    top_log_probs = _new(logits, (*lead, top), torch.float32)
-    top_tokens = _new(logits, (*lead, top), tokens.dtype)
+    shape = (*lead, top)
+    top_log_probs = _new(logits, shape, torch.float32)
+    top_tokens = _new(logits, shape, tokens.dtype)
     if n:
         held, space, need = _workspace(_N.log_probs_workspace(n, vocab), entropy.device)
         _call("pfa_token_log_probs", logits, rows.data_ptr(), stride, kind, n, vocab, tokens.data_ptr(), size, given, top,
