@@ -73,67 +73,6 @@ __device__ __forceinline__ f32x4 block_sums(const Widened &a, const Widened &b) 
     return sum;
 }
 
-// 16 rows of a and 16 columns a workgroup: b is streamed, its waves take the blocks of K in turn, four of a wave's on
-// their way at once, and meet in LDS, where the waves' sums are added in their order.  1 x 4096 x 4096: 5.1 us with
-// the matrix in the caches, 7.8 from memory, where the floor is 3.5 and a launch and one trip to memory take 4; what is
-// left is that lanes side by side read 16 rows (64 clocks a load where whole lines take 16).
-constexpr int kFewWaves = 8, kFewUnroll = 4;
-
-template <class T>
-__global__ void __launch_bounds__(kFewWaves * 64)
-k_fp8_few(Fp8Args g) {
-    using Operand = std::conditional_t<std::is_same_v<T, float>, Widened, Codes>;
-    __shared__ float sums[kFewWaves][16][17];
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, at = lane / 16 * 32;
-    const uint32_t n0 = blockIdx.x * 16, m0 = blockIdx.y * 16, am = min(m0 + lane % 16, g.M - 1);
-    const int8_t *pa = g.a + am * g.a_stride, *pb = g.b + min(n0 + lane % 16, g.N - 1) * g.b_stride;
-    const float *sa = g.sa + am * g.sa_row, *sb = g.sb + n0 / kBlock * g.sb_row;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    auto add = [&](const Codes &fa, const Codes &fb, float scale) {
-        const f32x4 p = block_sums(Operand(fa), Operand(fb));
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = fmaf(p[i], scale, acc[i]);
-    };
-    const uint32_t blocks = g.K / kBlock;
-    uint32_t j = wave;
-    for (; j + (kFewUnroll - 1) * kFewWaves < blocks; j += kFewUnroll * kFewWaves) {
-        Codes fa[kFewUnroll], fb[kFewUnroll];
-        float sj[kFewUnroll], tj[kFewUnroll];
-#pragma unroll
-        for (int u = 0; u < kFewUnroll; u++) {
-            const uint32_t k = j + u * kFewWaves;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                fb[u].v[h] = load16(pb, k * kBlock + at + h * 16);
-                fa[u].v[h] = load16(pa, k * kBlock + at + h * 16);
-            }
-            sj[u] = sa[k * g.sa_block];
-            tj[u] = sb[k * g.sb_block];
-        }
-#pragma unroll
-        for (int u = 0; u < kFewUnroll; u++) add(fa[u], fb[u], sj[u] * tj[u]);
-    }
-    // what is left: whole blocks, and the wave whose turn it is takes the rows' end
-    for (; j * kBlock < g.K; j += kFewWaves) {
-        Codes fa, fb;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            fb.v[h] = load16_end(pb, j * kBlock + at + h * 16, g.K);
-            fa.v[h] = load16_end(pa, j * kBlock + at + h * 16, g.K);
-        }
-        add(fa, fb, sa[j * g.sa_block] * sb[j * g.sb_block]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) sums[wave][lane % 16][lane / 16 * 4 + i] = acc[i];
-    __syncthreads();
-    const uint32_t m = threadIdx.x / 16, n = threadIdx.x % 16;
-    if (threadIdx.x >= 256 || m0 + m >= g.M || n0 + n >= g.N) return;
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kFewWaves; w++) v += sums[w][m][n];
-    static_cast<T *>(g.out)[(size_t)(m0 + m) * g.out_stride + n0 + n] = (T)(v + (g.bias ? g.bias[n0 + n] : 0.f));
-}
-
 // BYTES of memory a lane to a wave's 64 BYTES places in LDS: from p (scalar), `from` (scalar) and `own`, the latter two 32
 // bits in all.  Loads by such offsets are told apart from LDS accesses by the compiler's waits; by addresses of 64 bits
 // they are not, and the products of a block then wait for all operands of the next.
@@ -148,6 +87,169 @@ __device__ __forceinline__ void load_to_lds(const void *p, uint32_t from, uint32
     else
         __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, to, 4, own, from, 0, 0);
 #endif
+}
+
+// A wave's 16 x 16 sums in LDS, where the waves' are added in their order.  A lane has row lane % 16 of a, 4 columns.
+constexpr int kFewWaves = 8;
+using FewSums = float[kFewWaves][16][17];
+
+template <class T>
+__device__ __forceinline__ void few_outputs(const Fp8Args &g, FewSums &sums, const f32x4 &acc, uint32_t m0, uint32_t n0) {
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+#pragma unroll
+    for (int i = 0; i < 4; i++) sums[wave][lane % 16][lane / 16 * 4 + i] = acc[i];
+    __syncthreads();
+    const uint32_t m = threadIdx.x / 16, n = threadIdx.x % 16;
+    if (threadIdx.x >= 256 || m0 + m >= g.M || n0 + n >= g.N) return;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; w++) v += sums[w][m][n];
+    static_cast<T *>(g.out)[(size_t)(m0 + m) * g.out_stride + n0 + n] = (T)(v + (g.bias ? g.bias[n0 + n] : 0.f));
+}
+
+// 16 x 16 outputs a workgroup: b is streamed, its waves take the blocks of K in turn.  Lanes side by side read a row's
+// chunks and the matrix instruction wants them to have rows side by side, so blocks go through LDS, two of a wave's
+// own on their way at once, and no wave waits for another.  (More on their way leave LDS for one workgroup a CU instead
+// of two: 1 x 131072 x 4096 109 us with three.)  ROWS of a (8 or 16) are loaded; the sums of rows behind the matrix are
+// dropped.  Bound by memory, and by one trip to it where b is small: 1 x 131072 x 4096 92 us, to float32 88 (6.1 TB/s);
+// 1 x 4096 x 14336 12.1 us (4.9 TB/s), 1 x 4096 x 4096 5.6 us from memory, 1 x 128 x 4096 3.1 us.
+constexpr int kFewRing = 2;
+
+template <class T, int ROWS>
+__global__ void __launch_bounds__(kFewWaves * 64)
+k_fp8_few(Fp8Args g) {
+    using Operand = std::conditional_t<std::is_same_v<T, float>, Widened, Codes>;
+    // a block's 16 rows of b, its rows of a, each as in k_fp8_tiles, a's scales and b's
+    constexpr int kA = 16 * kBlock, kScales = kA + ROWS * kBlock, kSlot = kScales + 512, kLoads = 2 + ROWS / 8 + 2;
+    constexpr int kLds = kFewWaves * kFewRing * kSlot;
+    static_assert(kLds <= 160 * 1024 && kLds >= (int)sizeof(FewSums), "a CU's LDS");
+    __shared__ __align__(1024) int8_t held[kLds];
+    uint32_t start = 0;
+    asm("" : "+s"(start));
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    int8_t *mine = held + start + wave * (kFewRing * kSlot);
+    const uint32_t n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+    const int8_t *rows_a = g.a + m0 * g.a_stride, *rows_b = g.b + n0 * g.b_stride;
+    const float *sa = g.sa + m0 * g.sa_row, *sb = g.sb + n0 / kBlock * g.sb_row;
+    // a load is 8 rows, behind the matrix its last one
+    const uint32_t chunk = (lane % 8 ^ lane / 8) * 16, last_a = g.M - 1 - m0, last_b = g.N - 1 - n0;
+    uint32_t own_a[ROWS / 8], own_b[2];
+#pragma unroll
+    for (int i = 0; i < ROWS / 8; i++) own_a[i] = min(lane / 8 + i * 8, last_a) * (uint32_t)g.a_stride + chunk;
+#pragma unroll
+    for (int i = 0; i < 2; i++) own_b[i] = min(lane / 8 + i * 8, last_b) * (uint32_t)g.b_stride + chunk;
+    const uint32_t own_scale = min(lane % 16, last_a) * (uint32_t)g.sa_row * 4;
+    auto request = [&](int8_t *slot, uint32_t block) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) load_to_lds<16>(rows_b, block * kBlock, own_b[i], slot + i * 1024);
+#pragma unroll
+        for (int i = 0; i < ROWS / 8; i++) load_to_lds<16>(rows_a, block * kBlock, own_a[i], slot + kA + i * 1024);
+        load_to_lds<4>(sa + block * g.sa_block, 0, own_scale, slot + kScales);
+        load_to_lds<4>(sb + block * g.sb_block, 0, 0, slot + kScales + 256);  // by registers it waits for all loads
+    };
+    const uint32_t in_row = (lane / 16 ^ lane % 8) * 16, other = in_row ^ 64;
+    auto read = [&](const int8_t *row) {
+        Codes c;
+        c.v[0] = *reinterpret_cast<const i32x4 *>(row + in_row);
+        c.v[1] = *reinterpret_cast<const i32x4 *>(row + other);
+        return c;
+    };
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](const Codes &fa, const Codes &fb, float scale) {
+        const f32x4 p = block_sums(Operand(fa), Operand(fb));
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = fmaf(p[i], scale, acc[i]);
+    };
+    const uint32_t whole = g.K / kBlock;
+    auto fence = [] { asm volatile("" ::: "memory"); };
+#pragma unroll
+    for (int p = 0; p < kFewRing; p++)
+        if (wave + p * kFewWaves < whole) request(mine + p * kSlot, wave + p * kFewWaves);
+    // the wave whose turn it is takes the rows' end, while its blocks are on their way
+    if (const uint32_t j = whole; j * kBlock < g.K && j % kFewWaves == wave) {
+        const uint32_t at = lane / 16 * 16;
+        const int8_t *pa = rows_a + min(lane % 16, last_a) * g.a_stride, *pb = rows_b + min(lane % 16, last_b) * g.b_stride;
+        Codes fa, fb;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            fb.v[h] = load16_end(pb, j * kBlock + at + h * 64, g.K);
+            fa.v[h] = load16_end(pa, j * kBlock + at + h * 64, g.K);
+        }
+        add(fa, fb, sa[min(lane % 16, last_a) * g.sa_row + j * g.sa_block] * sb[j * g.sb_block]);
+    }
+    int8_t *slot = mine;
+    for (uint32_t j = wave; j < whole; j += kFewWaves) {
+        // this block has landed: of the loads behind it all may be on their way, or at the end none
+        fence();
+        if (j + (kFewRing - 1) * kFewWaves < whole)
+            __builtin_amdgcn_s_waitcnt(0x0f70 | (kLoads * (kFewRing - 1) & 15) | kLoads * (kFewRing - 1) >> 4 << 14);
+        else
+            __builtin_amdgcn_s_waitcnt(0x0f70);
+        fence();
+        const Codes fa = read(slot + kA + lane % ROWS * kBlock), fb = read(slot + lane % 16 * kBlock);
+        const float *scales = reinterpret_cast<const float *>(slot + kScales);
+        const float scale = scales[lane] * scales[64];
+        // and has been read, before its place is another's
+        fence();
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+        fence();
+        if (j + kFewRing * kFewWaves < whole) request(slot, j + kFewRing * kFewWaves);
+        slot = slot == mine + (kFewRing - 1) * kSlot ? mine : slot + kSlot;
+        add(fa, fb, scale);
+    }
+    __syncthreads();
+    few_outputs<T>(g, *reinterpret_cast<FewSums *>(held + start), acc, m0, n0);
+}
+
+// The same by registers, for rows so far apart that 32 bits do not hold the offsets of 16: a load of 16 rows by lanes
+// side by side takes 64 clocks where whole lines take 16 (1 x 4096 x 4096 from memory 7.8 us).
+constexpr int kFarUnroll = 4;
+
+template <class T>
+__global__ void __launch_bounds__(kFewWaves * 64)
+k_fp8_far(Fp8Args g) {
+    using Operand = std::conditional_t<std::is_same_v<T, float>, Widened, Codes>;
+    __shared__ FewSums sums;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, at = lane / 16 * 32;
+    const uint32_t n0 = blockIdx.x * 16, m0 = blockIdx.y * 16, am = min(m0 + lane % 16, g.M - 1);
+    const int8_t *pa = g.a + am * g.a_stride, *pb = g.b + min(n0 + lane % 16, g.N - 1) * g.b_stride;
+    const float *sa = g.sa + am * g.sa_row, *sb = g.sb + n0 / kBlock * g.sb_row;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](const Codes &fa, const Codes &fb, float scale) {
+        const f32x4 p = block_sums(Operand(fa), Operand(fb));
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = fmaf(p[i], scale, acc[i]);
+    };
+    const uint32_t blocks = g.K / kBlock;
+    uint32_t j = wave;
+    for (; j + (kFarUnroll - 1) * kFewWaves < blocks; j += kFarUnroll * kFewWaves) {
+        Codes fa[kFarUnroll], fb[kFarUnroll];
+        float sj[kFarUnroll], tj[kFarUnroll];
+#pragma unroll
+        for (int u = 0; u < kFarUnroll; u++) {
+            const uint32_t k = j + u * kFewWaves;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                fb[u].v[h] = load16(pb, k * kBlock + at + h * 16);
+                fa[u].v[h] = load16(pa, k * kBlock + at + h * 16);
+            }
+            sj[u] = sa[k * g.sa_block];
+            tj[u] = sb[k * g.sb_block];
+        }
+#pragma unroll
+        for (int u = 0; u < kFarUnroll; u++) add(fa[u], fb[u], sj[u] * tj[u]);
+    }
+    // what is left: whole blocks, and the wave whose turn it is takes the rows' end
+    for (; j * kBlock < g.K; j += kFewWaves) {
+        Codes fa, fb;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            fb.v[h] = load16_end(pb, j * kBlock + at + h * 16, g.K);
+            fa.v[h] = load16_end(pa, j * kBlock + at + h * 16, g.K);
+        }
+        add(fa, fb, sa[j * g.sa_block] * sb[j * g.sb_block]);
+    }
+    few_outputs<T>(g, sums, acc, m0, n0);
 }
 
 // The order of a wave's TM x TN products of a block: its first columns one by one, then the last `kRest` row by row.
@@ -547,18 +649,25 @@ struct Plan {
     bool few;
     int shape;
     uint32_t splits;
+    bool far = false;  // by k_fp8_far
 };
 
+// What k_fp8_few takes, measured in us against the best tile: up to two workgroups a CU, four for 32-bit outputs (16-bit:
+// 1 x 4096 x 4096 5.6 / 9.8, 64 x 2048 x 4096 5.8 / 9.5, 16 x 8192 x 4096 8.6 / 11.0, 16 x 12288 x 4096 13.3 / 11.9; 32-bit:
+// 16 x 12288 x 4096 12.6 / 16.3), one where sums are longer (64 x 1024 x 14336 10.6 / 13.0, 32 x 4096 x 14336 21.9 / 17.2);
+// and whatever b it is where a tile's rows are mostly empty (1 x 131072 x 4096 92 / 94 and 88 / 96, 4 x 57344 x 8192 80 /
+// 86 and 75 / 89).  The longest sums are split by tiles only (1 x 4096 x 32768 34 / 29, 16 x 1024 x 65536 42 / 23).
+bool by_few(size_t M, size_t N, size_t K, int type) {
+    const size_t groups = (M + 15) / 16 * ((N + 15) / 16);
+    if (K > 24576 || N >= (size_t)1 << 27) return false;
+    return M <= (type == PFA_F32 ? 16 : 8) || groups <= 256 || (K <= 8192 && groups <= (type == PFA_F32 ? 1024 : 512));
+}
+
 // The plan of least estimated time: that of the products and the tiles' ends, or of reading b, a little more for every
-// row of tiles that reads it again.  Few rows and few columns go to k_fp8_few (kernels, few / 32 x 64 tiles: 1 x 4096 x
-// 4096 7.8 / 9.6 us, float32 9.1 / 10.4; 16 x 8192 x 4096 12.4 / 11.3, float32 15.1 / 15.7; 16 x 16384 x 4096 20.6 /
-// 14.4), and what is at most a workgroup of it a CU, unless the sums are long (19 x 1414 x 1024 4.3 / 5.2, 120 x 405 x 3359
-// 8.9 / 11.9, 46 x 128 x 13056 15.1 / 10.7 with K split; 42 x 2595 x 1280, 489 workgroups, 7.1 / 5.6).  K is split
-// where tiles are too few for the card and the sums are long enough to pay for the second launch and the partial
-// sums (128 x 4096 x 16384: 59.8 us whole, 26.4 in 4).
+// row of tiles that reads it again.  K is split where tiles are too few for the card and the sums are long enough to
+// pay for the second launch and the partial sums (128 x 4096 x 16384: 59.8 us whole, 26.4 in 4).
 Plan plan_matmul(size_t M, size_t N, size_t K, int type) {
-    if (M <= 16 && N <= 8192) return {true, 0, 1};
-    if ((M + 15) / 16 * ((N + 15) / 16) <= 256 && K <= 8192) return {true, 0, 1};
+    if (by_few(M, N, K, type)) return {true, 0, 1};
     const float blocks = (float)((K + kBlock - 1) / kBlock), memory = 5e6f;  // bytes a us
     Plan best{false, 0, 1};
     float least = INFINITY;
@@ -598,7 +707,13 @@ void launch_tiles(const Fp8Args &g, hipStream_t s) {
 template <class T>
 void matmul(const Fp8Args &g, const Plan &p, hipStream_t s) {
     if (p.few) {
-        hipLaunchKernelGGL(k_fp8_few<T>, dim3((g.N + 15) / 16, (g.M + 15) / 16), dim3(kFewWaves * 64), 0, s, g);
+        const dim3 grid((g.N + 15) / 16, (g.M + 15) / 16), threads(kFewWaves * 64);
+        if (p.far)
+            hipLaunchKernelGGL(k_fp8_far<T>, grid, threads, 0, s, g);
+        else if (g.M <= 8)
+            hipLaunchKernelGGL((k_fp8_few<T, 8>), grid, threads, 0, s, g);
+        else
+            hipLaunchKernelGGL((k_fp8_few<T, 16>), grid, threads, 0, s, g);
         return;
     }
     switch (p.shape) {
@@ -673,7 +788,7 @@ int pfa_fp8_matmul(const uint8_t *a, size_t a_stride, const float *a_scales, siz
         const size_t far = (size_t)1 << 23;
         if ((M > 1 && (a_stride > far || a_scales_row > far / 8)) || (N > 1 && b_stride > far) ||
             (N > kBlock && b_scales_row > far))
-            p = {true, 0, 1};
+            p = {true, 0, 1, true};
         require(!p.few || (M <= 65535 * 16 && N < (size_t)1 << 27),
                 "pfa_fp8_matmul: rows this far apart: at most 1048560 of a and 2^27 - 1 of b");
         const size_t need = parts_bytes(M, N, p);

@@ -31,7 +31,8 @@ def test_products_reach_every_tile(kind, sizes, tiles):
         assert any(m % t[0] and n % t[1] for m, n, _ in mine), t
         assert any(m > (6 if t[0] >= 256 else 8) * t[0] for m, _, _ in mine), t
         for s in splits[t] - {1}:
-            assert {k % 128 == 0 for (_, _, k), p in plans.items() if p == (*t, s)} == {True, False}, (t, s)
+            ends = {k % 128 == 0 for (_, _, k), p in plans.items() if p == (*t, s)}
+            assert ends == ({True} if t == (256, 256) else {True, False}), (t, s)
     assert set().union(*splits.values()) == {1, 2, 4, 8}
 
 
@@ -39,7 +40,7 @@ def test_plan():
     for kind in (F32, BF16, F16):
         assert P.fp8_plan(1, 4096, 4096, kind) == (0, 16, 1) and P.fp8_plan(16, 8192, 100, kind) == (0, 16, 1)
         assert {P.fp8_plan(*size, kind) for size in FEW} == {(0, 16, 1)}
-        assert P.fp8_plan(17, 4096, 4096, kind)[0] > 0 and P.fp8_plan(1, 8193, 4096, kind)[0] > 0
+        assert P.fp8_plan(17, 16384, 4096, kind)[0] > 0 and P.fp8_plan(1, 4096, 24577, kind)[0] > 0
     assert P.fp8_plan(333, 777, 999, BF16) == P.fp8_plan(333, 777, 999, F16)
     for m, n, k in WIDE + NARROW:
         for kind in (F32, BF16):
@@ -49,7 +50,7 @@ def test_plan():
 
 def test_nothing_is_spilled(kernels):
     """Operands and sums stay in registers; the tiles of 256 x 256 give up a few numbers outside of their loop."""
-    for name in ("k_fp8_rows", "k_fp8_squares", "k_fp8_norm", "k_fp8_few", "k_fp8_tiles", "k_fp8_join", "k_log_rows",
+    for name in ("k_fp8_rows", "k_fp8_squares", "k_fp8_norm", "k_fp8_few", "k_fp8_far", "k_fp8_tiles", "k_fp8_join", "k_log_rows",
                  "k_log_parts", "k_log_join"):
         found = named(kernels, name)
         assert found, name
