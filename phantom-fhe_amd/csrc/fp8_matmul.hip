@@ -652,6 +652,8 @@ struct Plan {
     bool far = false;  // by k_fp8_far
 };
 
+constexpr size_t kFewColumns = (size_t)1 << 26;  // a launch of k_fp8_few has 2^32 threads at twice as many
+
 // What k_fp8_few takes, measured in us against the best tile: up to two workgroups a CU, four for 32-bit outputs (16-bit:
 // 1 x 4096 x 4096 5.6 / 9.8, 64 x 2048 x 4096 5.8 / 9.5, 16 x 8192 x 4096 8.6 / 11.0, 16 x 12288 x 4096 13.3 / 11.9; 32-bit:
 // 16 x 12288 x 4096 12.6 / 16.3), one where sums are longer (64 x 1024 x 14336 10.6 / 13.0, 32 x 4096 x 14336 21.9 / 17.2);
@@ -659,7 +661,7 @@ struct Plan {
 // 86 and 75 / 89).  The longest sums are split by tiles only (1 x 4096 x 32768 34 / 29, 16 x 1024 x 65536 42 / 23).
 bool by_few(size_t M, size_t N, size_t K, int type) {
     const size_t groups = (M + 15) / 16 * ((N + 15) / 16);
-    if (K > 24576 || N >= (size_t)1 << 27) return false;
+    if (K > 24576 || N >= kFewColumns) return false;
     return M <= (type == PFA_F32 ? 16 : 8) || groups <= 256 || (K <= 8192 && groups <= (type == PFA_F32 ? 1024 : 512));
 }
 
@@ -789,8 +791,8 @@ int pfa_fp8_matmul(const uint8_t *a, size_t a_stride, const float *a_scales, siz
         if ((M > 1 && (a_stride > far || a_scales_row > far / 8)) || (N > 1 && b_stride > far) ||
             (N > kBlock && b_scales_row > far))
             p = {true, 0, 1, true};
-        require(!p.few || (M <= 65535 * 16 && N < (size_t)1 << 27),
-                "pfa_fp8_matmul: rows this far apart: at most 1048560 of a and 2^27 - 1 of b");
+        require(!p.few || (M <= 65535 * 16 && N < kFewColumns),
+                "pfa_fp8_matmul: rows this far apart: at most 1048560 of a and 2^26 - 1 of b");
         const size_t need = parts_bytes(M, N, p);
         require(workspace_bytes >= need, "pfa_fp8_matmul: the workspace needs " + std::to_string(need) + " bytes");
         require(((uintptr_t)workspace & 15) == 0, "pfa_fp8_matmul: the workspace is not aligned to 16 bytes");

@@ -40,6 +40,7 @@ def test_plan():
     for kind in (F32, BF16, F16):
         assert P.fp8_plan(1, 4096, 4096, kind) == (0, 16, 1) and P.fp8_plan(16, 8192, 100, kind) == (0, 16, 1)
         assert {P.fp8_plan(*size, kind) for size in FEW} == {(0, 16, 1)}
+        assert P.fp8_plan(1, (1 << 26) - 1, 128, kind) == (0, 16, 1) and P.fp8_plan(1, 1 << 26, 128, kind)[0] > 0  # a grid's end
         assert P.fp8_plan(17, 16384, 4096, kind)[0] > 0 and P.fp8_plan(1, 4096, 24577, kind)[0] > 0
     assert P.fp8_plan(333, 777, 999, BF16) == P.fp8_plan(333, 777, 999, F16)
     for m, n, k in WIDE + NARROW:

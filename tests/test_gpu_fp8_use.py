@@ -225,6 +225,24 @@ def test_outputs_past_32_bits(dev):
     assert int((out != 0).sum()) == 4
 
 
+def test_most_columns(dev):
+    """A token and as many columns as one launch without tiles forms, and one more; b has 2^33 bytes."""
+    import torch
+
+    k = 128
+    one = torch.ones((1, k), device=dev).to(torch.float8_e4m3fn)
+    sa = torch.full((1, 1), 2.0, device=dev)
+    for n in ((1 << 26) - 1, 1 << 26):
+        b = torch.zeros((n, k), dtype=torch.uint8, device=dev)
+        b[-1], b[0], b[(1 << 25) + 5] = one.view(torch.uint8), one.view(torch.uint8), one.view(torch.uint8)
+        sb = torch.ones((R.spans(n), 1), device=dev)
+        sb[-1] = 3
+        out = ph.fp8_matmul(one, sa, b.view(torch.float8_e4m3fn), sb, None, torch.float16)
+        assert out[0, -1] == 6 * k and out[0, 0] == 2 * k and out[0, (1 << 25) + 5] == 2 * k
+        assert int((out != 0).sum()) == 3
+        del b, out
+
+
 def test_example(dev):
     """examples/encrypted_decoding.py with the vocabulary in 8-bit floats runs, and says the tokens it kept."""
     import importlib.util
