@@ -656,6 +656,7 @@ struct Plan {
 };
 
 constexpr size_t kFewColumns = (size_t)1 << 26;  // a launch of k_fp8_few has 2^32 threads at twice as many
+constexpr size_t kMostTiles = (size_t)1 << 22;   // a launch of 512 threads a tile has 2^32 at twice as many
 
 // What k_fp8_few takes, measured in us against the best tile: up to two workgroups a CU, four for 32-bit outputs (16-bit:
 // 1 x 4096 x 4096 5.6 / 9.8, 64 x 2048 x 4096 5.8 / 9.5, 16 x 8192 x 4096 8.6 / 11.0, 16 x 12288 x 4096 13.3 / 11.9; 32-bit:
@@ -674,34 +675,39 @@ bool by_few(size_t M, size_t N, size_t K, int type) {
 Plan plan_matmul(size_t M, size_t N, size_t K, int type) {
     if (by_few(M, N, K, type)) return {true, 0, 1};
     const float blocks = (float)((K + kBlock - 1) / kBlock), memory = 5e6f;  // bytes a us
-    Plan best{false, 0, 1};
+    Plan best{false, -1, 1};
     float least = INFINITY;
-    for (int i = 0; i < kShapes; i++) {
-        const Shape &s = shapes[i];
-        if (s.rows > 32 && M <= s.rows / 2) continue;                 // half a tile or more of nothing
-        if (i == kVast && (type == PFA_F32 || K % kBlock)) continue;  // takes whole blocks only
-        const Cost &c = type == PFA_F32 ? s.wide : s.narrow;
-        const size_t down = (M + s.rows - 1) / s.rows, tiles = down * ((N + s.cols - 1) / s.cols);
-        const float reading = ((float)N * K * (1 + .15f * (down - 1)) + (float)M * K) / memory;
-        for (uint32_t splits = 1; splits <= 8; splits *= 2) {
-            if (splits > 1 && (tiles * splits > 512 || blocks < 8 * splits)) break;
-            const size_t on_cu = (tiles * splits + 255) / 256;
-            const float block = on_cu <= 1 ? c.alone : on_cu == 2 ? c.pair : on_cu * c.each;
-            const float join = splits == 1 ? 0.f : 4.f + (float)splits * M * N * 8 / memory;
-            const float time = std::max(block * blocks / splits + on_cu * c.end, reading) + join;
-            if (time < least) {
-                least = time;
-                best = {false, i, splits};
+    auto look = [&](bool half_empty) {
+        for (int i = 0; i < kShapes; i++) {
+            const Shape &s = shapes[i];
+            if (s.rows > 32 && M <= s.rows / 2 && !half_empty) continue;  // half a tile or more of nothing
+            if (i == kVast && (type == PFA_F32 || K % kBlock)) continue;  // takes whole blocks only
+            const Cost &c = type == PFA_F32 ? s.wide : s.narrow;
+            const size_t down = (M + s.rows - 1) / s.rows, tiles = down * ((N + s.cols - 1) / s.cols);
+            if (tiles >= kMostTiles) continue;
+            const float reading = ((float)N * K * (1 + .15f * (down - 1)) + (float)M * K) / memory;
+            for (uint32_t splits = 1; splits <= 8; splits *= 2) {
+                if (splits > 1 && (tiles * splits > 512 || blocks < 8 * splits)) break;
+                const size_t on_cu = (tiles * splits + 255) / 256;
+                const float block = on_cu <= 1 ? c.alone : on_cu == 2 ? c.pair : on_cu * c.each;
+                const float join = splits == 1 ? 0.f : 4.f + (float)splits * M * N * 8 / memory;
+                const float time = std::max(block * blocks / splits + on_cu * c.end, reading) + join;
+                if (time < least) {
+                    least = time;
+                    best = {false, i, splits};
+                }
             }
         }
-    }
+    };
+    look(false);
+    if (best.shape < 0) look(true);  // a few rows of more columns than low tiles cover
+    require(best.shape >= 0, "pfa_fp8_matmul: more outputs than one launch can form");
     return best;
 }
 
 template <class T, int BM, int BN, int WM, int WN, int STAGES>
 void launch_tiles(const Fp8Args &g, hipStream_t s) {
-    const size_t jobs = (size_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN) * g.splits;
-    require(jobs < 1u << 22, "pfa_fp8_matmul: more outputs than one launch can form");
+    const size_t jobs = (size_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN) * g.splits;  // below kMostTiles
     hipLaunchKernelGGL((k_fp8_tiles<T, BM, BN, WM, WN, STAGES>), dim3((uint32_t)((jobs + 7) / 8 * 8)), dim3(WM * WN * 64), 0,
                        s, g);
     if (g.splits > 1)
