@@ -1,10 +1,13 @@
-"""The largest products that fp8_matmul forms, and that all of its entry points refuse the same ones (no GPU needed)."""
+"""The largest products that fp8_matmul forms, that all of its entry points refuse the same ones, and the arithmetic of
+its 16-bit outputs (no GPU needed)."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 import pfa_native as P
 from test_clear_ops import _abi
+from test_gpu_fp8_precision import aligned_sum, power
 
 MOST = 1 << 22  # tiles of a launch
 KINDS = [0, 1, 2]
@@ -50,3 +53,17 @@ def test_rows_too_far_apart(kind):
         rc, words = _abi("pfa_fp8_matmul", p, a_stride, p, 1, m, p, b_stride, p, 1, 1, None, m, n, 128, p, kind, n, None, 0,
                          None)
         assert rc == P.PFA_ERR_INVALID_ARGUMENT and "far apart" in words, words
+
+
+def test_cut_is_no_more_than_stated():
+    """Seven of eight products can lose less than 2^-13 of the largest product of powers each; with subnormal codes that is
+    more than 2^-13 of the largest product itself."""
+    rng = np.random.default_rng(4)
+    worst = 0.0
+    for _ in range(2000):
+        a, b = (np.rint(rng.standard_normal(8) * 8) * np.exp2(rng.integers(-9, 6, 8)) for _ in range(2))
+        at = np.where(a * b != 0, power(a) * power(b), 0.0).max()
+        lost = abs(aligned_sum(a, b) - (a * b).sum())
+        assert lost <= 7 * 2.0 ** -13 * at
+        worst = max(worst, lost / (2.0 ** -13 * max(np.abs(a * b).max(), 1e-300)))
+    assert worst > 1

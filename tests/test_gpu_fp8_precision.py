@@ -80,20 +80,6 @@ def test_cut(dev, size):
         assert product(a, b, size, "float32", dev) == (a * b).sum(), name
 
 
-def test_cut_is_no_more_than_stated():
-    """Seven of eight products can lose less than 2^-13 of the largest product of powers each; with subnormal codes that is
-    more than 2^-13 of the largest product itself (no GPU needed for the arithmetic of the rule)."""
-    rng = np.random.default_rng(4)
-    worst = 0.0
-    for _ in range(2000):
-        a, b = (np.rint(rng.standard_normal(8) * 8) * np.exp2(rng.integers(-9, 6, 8)) for _ in range(2))
-        at = np.where(a * b != 0, power(a) * power(b), 0.0).max()
-        lost = abs(aligned_sum(a, b) - (a * b).sum())
-        assert lost <= 7 * 2.0 ** -13 * at
-        worst = max(worst, lost / (2.0 ** -13 * max(np.abs(a * b).max(), 1e-300)))
-    assert worst > 1
-
-
 @pytest.mark.parametrize("m,n,k", [(1, 512, 4096), (64, 512, 4096), (300, 700, 2050), (200, 2000, 1024)])
 @pytest.mark.parametrize("dtype", NARROW)
 def test_ordinary_outputs(dev, dtype, m, n, k):
