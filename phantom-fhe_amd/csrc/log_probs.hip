@@ -80,17 +80,6 @@ struct Running {
         }
         return m;
     }
-    __device__ __forceinline__ void join(float other_top, float other_sum, float other_turn, const Heat &heat) {
-        Running o;
-        o.top = other_top;
-        o.sum = other_sum;
-        o.turn = other_turn;
-        const float m = fmaxf(top, o.top);
-        lift(m, heat);
-        o.lift(m, heat);
-        sum += o.sum;
-        turn += o.turn;
-    }
 };
 
 // A row's logits, and which of its places are allowed.  MASKED: a call without a mask has no code for one in its loop.
