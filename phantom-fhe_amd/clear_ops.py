@@ -416,8 +416,8 @@ def token_log_probs(logits, tokens, top=0, temperature=1.0, mask=None):
     float32 like tokens, entropy float32 [...], top_log_probs float32 [..., top], top_tokens
     [..., top] of tokens' type).
 
-    logits [..., vocab]; tokens int32 or int64, [...] (one for each row) or [..., given];
-    temperature and mask as for token_probabilities; natural logarithms.  The alternatives are
+    logits [..., vocab]; tokens int32 or int64, contiguous, [...] (one for each row) or [..., given];
+    temperature (contiguous too) and mask as for token_probabilities; natural logarithms.  The alternatives are
     the `top` (64 at most) allowed places of the largest logits, larger ones first, the lowest
     place first among equals.  A token outside the vocabulary (padding) or not allowed has
     -infinity; where fewer than `top` places are allowed (with a logit above -infinity), -1 and
