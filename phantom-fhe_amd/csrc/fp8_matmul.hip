@@ -114,8 +114,8 @@ __device__ __forceinline__ void few_outputs(const Fp8Args &g, FewSums &sums, con
 // chunks and the matrix instruction wants them to have rows side by side, so blocks go through LDS, two of a wave's
 // own on their way at once, and no wave waits for another.  (More on their way leave LDS for one workgroup a CU instead
 // of two: 1 x 131072 x 4096 109 us with three.)  ROWS of a (8 or 16) are loaded; the sums of rows behind the matrix are
-// dropped.  Bound by memory, and by one trip to it where b is small: 1 x 131072 x 4096 92 us, to float32 88 (6.1 TB/s);
-// 1 x 4096 x 14336 12.1 us (4.9 TB/s), 1 x 4096 x 4096 5.6 us from memory, 1 x 128 x 4096 3.1 us.
+// dropped.  Bound by memory: 1 x 131072 x 4096 92 us, to float32 88 (6.1 TB/s); 1 x 4096 x 14336 12.1 us (4.9 TB/s),
+// 1 x 4096 x 4096 5.6 us from memory.  Where b is small by the launch and one trip to memory: 1 x 128 x 4096 3.1 us.
 constexpr int kFewRing = 2;
 
 template <class T, int ROWS>
