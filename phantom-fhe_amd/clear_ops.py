@@ -356,10 +356,11 @@ def fp8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
     where a few places of a are 200 times the others, 1.9e-4 at most in the mean square, beside
     the 1.7e-3 (bfloat16) or 2e-4 (float16) of the output's own rounding.  Where large products
     cancel, the small ones cut beside them are missing.  For float32 outputs every product counts
-    whole, at up to half the speed where the product is not bound by reading b.  Rows of a and b
-    that start at multiples of 128 bytes are read fastest, and a_scales whose values of one block
-    stand together.  Outputs that take 2^22 tiles of 128 x 256 and of 256 x 128 or more (2^37 of
-    them; a row or a column of 2^30) are refused.
+    whole, at about half the speed where the product is not bound by reading b; converted
+    afterwards they are 16-bit outputs without the cut.  Rows of a and b that start at multiples of
+    128 bytes are read fastest, and a_scales whose values of one block stand together.  Outputs that
+    take 2^22 tiles of 128 x 256 and of 256 x 128 or more (2^37 of them; a row or a column of 2^30)
+    are refused.
     """
     kind = _TYPE.get(out_dtype)
     if kind is None:
