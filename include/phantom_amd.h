@@ -516,9 +516,10 @@ int pfa_fp8_plan(size_t M, size_t N, size_t K, int type, size_t *tile_rows, size
  * largest product of two codes' powers of two (2^-6 for a code below it; of products that are not 0), it
  * cuts each to a multiple of 2^-13 P, towards 0, before it adds them.  For 32-bit outputs every product is
  * added whole.  workspace: pfa_fp8_workspace bytes, otherwise as in pfa_int8_matmul.
- * Refused, here and by pfa_fp8_workspace and pfa_fp8_plan: outputs that take 2^22 tiles of 128 x 256 and of
- * 256 x 128 or more (2^37 outputs; a row or a column of 2^30).  Where rows of a or b are more than 2^23 bytes apart, or
- * rows of scales more than 2^20 (a) or 2^23 (b) numbers: more than 1048560 rows of a or 2^26 - 1 of b. */
+ * Refused, here and by pfa_fp8_workspace and pfa_fp8_plan: outputs that take 2^22 tiles or more in every shape, the
+ * largest being 128 x 256 and 256 x 128 (2^37 outputs; a row or a column of 2^30), and 256 x 256 for 16-bit outputs of
+ * whole blocks.  Where rows of a or b are more than 2^23 bytes apart, or rows of scales more than 2^20 (a) or 2^23 (b)
+ * numbers: more than 1048560 rows of a or 2^26 - 1 of b. */
 int pfa_fp8_matmul(const uint8_t *a, size_t a_stride, const float *a_scales, size_t a_scales_row, size_t a_scales_block,
                    const uint8_t *b, size_t b_stride, const float *b_scales, size_t b_scales_row, size_t b_scales_block,
                    const float *bias, size_t M, size_t N, size_t K, void *out, int type, size_t out_stride,

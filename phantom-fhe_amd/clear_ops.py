@@ -358,9 +358,9 @@ def fp8_matmul(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16):
     cancel, the small ones cut beside them are missing.  For float32 outputs every product counts
     whole, at about half the speed where the product is not bound by reading b; converted
     afterwards they are 16-bit outputs without the cut.  Rows of a and b that start at multiples of
-    128 bytes are read fastest, and a_scales whose values of one block stand together.  Outputs that
-    take 2^22 tiles of 128 x 256 and of 256 x 128 or more (2^37 of them; a row or a column of 2^30)
-    are refused.
+    128 bytes are read fastest, and a_scales whose values of one block stand together.  Refused
+    are outputs that take 2^22 tiles or more in every shape, the largest being 128 x 256 and 256 x
+    128 (2^37 outputs; a row or a column of 2^30).
     """
     kind = _TYPE.get(out_dtype)
     if kind is None:
